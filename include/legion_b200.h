@@ -351,6 +351,79 @@ int legion_gather_rows_noalloc(void *stream, int32_t dev_id, const int32_t *ids_
                                const void *const *partitions, const void *host_table, int64_t n_nodes,
                                int32_t row_bytes, void *out_dev);
 
+/* ---- learned rows, norm and products ------------------------------------------------------------------ */
+
+/* Operators that a model needs next to the rows served above: lookup of learned rows with its gradient, RMS norm
+ * with its gradient, and products of compressed rows.  They work on device memory of dev_id, in the order of `stream`,
+ * allocate nothing, keep nothing between calls, do not synchronise, may be captured into a CUDA graph, and leave the calling
+ * thread's current device as it was.  Calls on different streams may run at the same time as long as they do
+ * not share a workspace or an output.  Rows are rows of dim elements; strides are in elements (compressed rows: in bytes) and may be
+ * longer than the row; what lies between rows is neither read nor written.  Addresses are multiples of the element's size; rows
+ * whose addresses, strides and length are multiples of 16 bytes move by the widest loads.  Results do not depend on the order in
+ * which the GPU runs its blocks: the same call gives the same bits. */
+#define LEGION_F32 0
+#define LEGION_F16 1
+#define LEGION_BF16 2
+#define LEGION_MAX_IDS (1 << 28)
+#define LEGION_MAX_DIM (1 << 16)
+#define LEGION_NORM_MAX_DIM (1 << 14)
+#define LEGION_MATMUL_MAX_DIM 131068 /* sums of products of two codes stay inside 32 bits */
+
+/* out[i] = scale * table[ids[i]], computed in fp32 and rounded once; an id outside [0, n_nodes) gives a row of zeros.
+ * ids: n_ids values of id_bytes (4 or 8) on the device; any id may come any number of times.  The gather of given rows is
+ * FeatureCacheLookup (engine/operator_impl.cuh:39-53); learned rows have no counterpart in the reference. */
+int legion_embedding_lookup(int32_t dev_id, const void *table, int32_t table_dtype, int64_t table_stride, int64_t n_nodes,
+                            const void *ids, int32_t id_bytes, int64_t n_ids, int32_t dim, float scale, void *out,
+                            int32_t out_dtype, int64_t out_stride, void *stream);
+/* Bytes of scratch of the two calls below.  The workspace starts on a multiple of 16 bytes, may hold anything, and serves one
+ * call at a time (a captured graph keeps using the one it was captured with). */
+int legion_embedding_grad_workspace(int64_t n_ids, int32_t dim, int64_t n_nodes, int64_t *bytes);
+/* The lookup's gradient: grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] = v (zeros for a row that no id names),
+ * or, accumulate != 0, that added to grad_table[v] (other rows stay as they are).  Sums are fp32, in an order that
+ * depends on the ids alone, rounded once.  Ids outside [0, n_nodes) are left out. */
+int legion_embedding_grad(int32_t dev_id, const void *ids, int32_t id_bytes, int64_t n_ids, const void *grad_out,
+                          int32_t grad_dtype, int64_t grad_stride, int32_t dim, float scale, void *grad_table,
+                          int32_t table_dtype, int64_t table_stride, int64_t n_nodes, int32_t accumulate, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+/* The same for a table that is too large to have a gradient of its size: unique_ids[0 .. *count) = the ids that occur, rising
+ * (as wide as ids), grad_rows[k] = the fp32 gradient of row unique_ids[k].  Both have room for n_ids entries; those behind *count
+ * (one int32 on the device) are left as they were. */
+int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32_t id_bytes, int64_t n_ids, const void *grad_out,
+                               int32_t grad_dtype, int64_t grad_stride, int32_t dim, float scale, int64_t n_nodes,
+                               void *unique_ids, float *grad_rows, int64_t rows_stride, int32_t *count, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
+/* h = x + residual (residual may be NULL), out = h * weight / sqrt(mean(h^2) + eps) over rows of dim elements.  x, residual,
+ * residual_out (h rounded once; may be NULL) and, codec RAW, out are of `dtype`; weight is fp32 or of that type.  codec INT8 or E4M3:
+ * out receives compressed rows, out_stride bytes apart (a multiple of 16): dim codes, an fp32 scale, zeros up to a multiple of 16
+ * bytes, exactly what legion_quantize_table makes of the fp32 rows (dim % 4 == 0).  out and residual_out may be x or residual
+ * themselves (same address and stride), but not each other; other overlaps are not allowed.  h and its squares are fp32: a
+ * row whose squares sum to more than 3.4e38 has an infinite mean. */
+int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stride, const void *residual,
+                    int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim,
+                    int32_t codec, void *out, int64_t out_stride, void *residual_out, int64_t residual_out_stride, void *stream);
+int legion_rms_norm_grad_workspace(int64_t n_rows, int32_t dim, int64_t *bytes);
+/* The norm's gradient.  x: the rows that were normed (with a residual: residual_out).  grad_x = the gradient of x by way of out, plus
+ * grad_residual (the gradient that reached residual_out otherwise; may be NULL); with a residual it is the gradient
+ * of both.  grad_weight (dim elements, fp32 or the rows' type) is set, not added to.  grad_x may be grad_out, x or grad_residual.
+ * Workspace as above. */
+int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_t grad_stride, const void *x, int64_t x_stride,
+                         int32_t dtype, const void *grad_residual, int64_t grad_residual_stride, const void *weight,
+                         int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim, void *grad_x, int64_t grad_x_stride,
+                         void *grad_weight, int32_t grad_weight_dtype, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* out[i][j] = scale of row i * scale of weight row j * sum over k of their codes' products: m compressed rows (of legion_rms_norm,
+ * legion_quantize_table or a cache's partition) times n compressed weight rows (one per output column, for instance
+ * legion_quantize_table of an fp32 weight [n][feature_len]), feature_len codes each, both of `codec`.  Strides in bytes, multiples of 16; rows start on
+ * multiples of 16 bytes.  int8 products are summed exactly, e4m3 products in fp32; the sum is scaled in fp32 and rounded once.
+ * Bytes of a row behind its scale are not read. */
+int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t m, int64_t row_stride, const void *weight_rows,
+                       int64_t n, int64_t weight_stride, int32_t feature_len, void *out, int32_t out_dtype, int64_t out_stride,
+                       void *stream);
+/* First error that a kernel of these operators raised on dev_id since the last reset (0: none; LEGION_E_TIMEOUT: a copy or a product
+ * inside legion_matmul_rows did not complete within its wait limit, the call's output is not valid).  Waits for `stream`. */
+int legion_operator_error(int32_t dev_id, void *stream, int32_t *error, int32_t reset);
+
 /* ---- whole batch --------------------------------------------------------------------- */
 
 /* The op list of GPURunner::RunOnce (engine/server.cu:342-351) for one batch on one stream set.

@@ -20,6 +20,7 @@ CODEC_RAW, CODEC_INT8, CODEC_E4M3 = 0, 1, 2
 (BUF_IDS, BUF_FEATURES, BUF_LABELS, BUF_AGG_SRC, BUF_AGG_DST, BUF_NODE_COUNTER, BUF_EDGE_COUNTER,
  BUF_CACHE_INDEX, BUF_SRC_GLOBAL) = range(9)
 INTRABATCH_CON = 3
+F32, F16, BF16 = range(3)
 
 _lib = None
 
@@ -46,6 +47,7 @@ def lib():
                               "(there is no CPU fallback)")
         _lib = C.CDLL(LIB_PATH)
         _lib.legion_last_error.restype = C.c_char_p
+        _declare_operators(_lib)
     return _lib
 
 
@@ -360,6 +362,190 @@ def gather_rows_noalloc(stream, dev_id, ids_dev, lut_ptr, capacity, kg, ki, part
                                             C.c_int64(ids_dev.numel()), C.c_void_p(lut_ptr), C.c_int32(capacity),
                                             C.c_int32(kg), C.c_int32(ki), parts, _ptr(host_table), C.c_int64(n_nodes),
                                             C.c_int32(row_bytes), _ptr(out_dev)))
+
+
+# ---- learned rows, norm and products ------------------------------------------------------------------
+
+def _declare_operators(l):
+    """Argument types of the operators that are called once per layer: plain numbers then need no wrapping per call."""
+    P, I, Q, F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+    l.legion_embedding_lookup.argtypes = [I, P, I, Q, Q, P, I, Q, I, F, P, I, Q, P]
+    l.legion_embedding_grad.argtypes = [I, P, I, Q, P, I, Q, I, F, P, I, Q, Q, I, P, Q, P]
+    l.legion_embedding_grad_rows.argtypes = [I, P, I, Q, P, I, Q, I, F, Q, P, P, Q, P, P, Q, P]
+    l.legion_embedding_grad_workspace.argtypes = [Q, I, Q, P]
+    l.legion_rms_norm.argtypes = [I, P, I, Q, P, Q, P, I, F, Q, I, I, P, Q, P, Q, P]
+    l.legion_rms_norm_grad.argtypes = [I, P, Q, P, Q, I, P, Q, P, I, F, Q, I, P, Q, P, I, P, Q, P]
+    l.legion_rms_norm_grad_workspace.argtypes = [Q, I, P]
+    l.legion_matmul_rows.argtypes = [I, I, P, Q, Q, P, Q, Q, I, P, I, Q, P]
+    l.legion_operator_error.argtypes = [I, P, P, I]
+
+
+_dtypes = {}
+
+
+def _code_of(dtype):
+    if not _dtypes:
+        import torch
+        _dtypes.update({torch.float32: (F32, 0), torch.float16: (F16, 0), torch.bfloat16: (BF16, 0), torch.int32: (-1, 4),
+                        torch.int64: (-1, 8), torch.uint8: (-1, 1)})
+    return _dtypes.get(dtype, (-1, 0))
+
+
+def _operand(what, t, dev_id, dims, shape=None):
+    """Type code of a float tensor, after the checks that a pointer cannot make: where it lies, its shape, whole rows."""
+    if t.dim() != dims or (shape is not None and tuple(t.shape) != shape):
+        raise LegionError("%s: shape %s, expected %s" % (what, tuple(t.shape), shape if shape is not None else "%d dimensions" % dims))
+    if not t.is_cuda or t.get_device() != dev_id:
+        raise LegionError("%s is on %s, the call is for cuda:%d" % (what, t.device, dev_id))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise LegionError("%s: the elements of a row must lie one behind the other" % what)
+    return _code_of(t.dtype)
+
+
+def _rows(what, t, dev_id, shape=None):
+    code = _operand(what, t, dev_id, 2, shape)[0]
+    if code < 0:
+        raise LegionError("%s: %s is not float32, float16 or bfloat16" % (what, t.dtype))
+    return code
+
+
+def _row_stride(t):
+    """Elements from row to row; one row (or none) has no next one."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _id_width(what, ids, dev_id):
+    code, width = _operand(what, ids, dev_id, 1)
+    if code >= 0 or width not in (4, 8):
+        raise LegionError("%s: %s is not int32 or int64" % (what, ids.dtype))
+    return width
+
+
+def _code_rows(what, t, dev_id, feature_len):
+    if _operand(what, t, dev_id, 2) != (-1, 1):
+        raise LegionError("%s: %s is not uint8" % (what, t.dtype))
+    need = (feature_len + 4 + 15) // 16 * 16
+    if t.shape[1] < need:
+        raise LegionError("%s: rows of %d bytes, compressed rows of %d codes have %d" % (what, t.shape[1], feature_len, need))
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), need) + 15 & -16
+
+
+def _workspace(t, dev_id):
+    if t is None:
+        return None, 0
+    if not t.is_cuda or t.get_device() != dev_id or not t.is_contiguous():
+        raise LegionError("workspace must be contiguous memory of cuda:%d" % dev_id)
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _handle(stream):
+    return None if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def embedding_lookup(dev_id, table, ids, out, scale=1.0, stream=None):
+    """out[i] = scale * table[ids[i]] for a table [nodes, dim] of learned rows; an id outside the table gives a row of zeros.
+    table and out: float32, float16 or bfloat16, each its own; ids: int32 or int64."""
+    td, od, width = _rows("table", table, dev_id), _rows("out", out, dev_id, (ids.shape[0], table.shape[1])), _id_width("ids", ids, dev_id)
+    _check(lib().legion_embedding_lookup(dev_id, table.data_ptr(), td, _row_stride(table), table.shape[0], ids.data_ptr(), width,
+                                         ids.shape[0], table.shape[1], scale, out.data_ptr(), od, _row_stride(out), _handle(stream)))
+
+
+def embedding_grad_workspace(n_ids, dim, n_nodes):
+    """Bytes of scratch that embedding_grad and embedding_grad_rows take for n_ids ids."""
+    b = C.c_int64()
+    _check(lib().legion_embedding_grad_workspace(n_ids, dim, n_nodes, C.byref(b)))
+    return b.value
+
+
+def embedding_grad(dev_id, ids, grad_out, grad_table, workspace, scale=1.0, accumulate=False, stream=None):
+    """grad_table[v] = scale * sum of grad_out[i] over ids[i] == v, or added to what grad_table holds.  Ids outside the table
+    are left out."""
+    gd, td, width = _rows("grad_out", grad_out, dev_id, (ids.shape[0], grad_table.shape[1])), _rows("grad_table", grad_table, dev_id), \
+        _id_width("ids", ids, dev_id)
+    ws, ws_bytes = _workspace(workspace, dev_id)
+    _check(lib().legion_embedding_grad(dev_id, ids.data_ptr(), width, ids.shape[0], grad_out.data_ptr(), gd, _row_stride(grad_out),
+                                       grad_table.shape[1], scale, grad_table.data_ptr(), td, _row_stride(grad_table),
+                                       grad_table.shape[0], 1 if accumulate else 0, ws, ws_bytes, _handle(stream)))
+
+
+def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, count, workspace, scale=1.0, stream=None):
+    """The gradient's rows that occur: unique_ids[:count] rising, grad_rows[:count] their float32 gradients; count is one
+    int32 on the device.  What lies behind count is left as it was."""
+    n, dim = grad_out.shape
+    gd, width = _rows("grad_out", grad_out, dev_id, (ids.shape[0], dim)), _id_width("ids", ids, dev_id)
+    if _rows("grad_rows", grad_rows, dev_id) != F32 or grad_rows.shape[0] < n or grad_rows.shape[1] != dim:
+        raise LegionError("grad_rows must be float32, with a row for every id")
+    if _id_width("unique_ids", unique_ids, dev_id) != width or unique_ids.shape[0] < n:
+        raise LegionError("unique_ids must be as wide as ids, with an entry for every id")
+    if _operand("count", count, dev_id, 1, (1,)) != (-1, 4):
+        raise LegionError("count must be one int32")
+    ws, ws_bytes = _workspace(workspace, dev_id)
+    _check(lib().legion_embedding_grad_rows(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, _row_stride(grad_out), dim, scale,
+                                            n_nodes, unique_ids.data_ptr(), grad_rows.data_ptr(), _row_stride(grad_rows),
+                                            count.data_ptr(), ws, ws_bytes, _handle(stream)))
+
+
+def rms_norm(dev_id, x, weight, out, eps=1e-6, residual=None, residual_out=None, codec=CODEC_RAW, stream=None):
+    """h = x + residual; out = h * weight / sqrt(mean(h^2) + eps); residual_out = h.  codec CODEC_INT8 or CODEC_E4M3: out is uint8
+    and receives the compressed rows that quantize_table would make of the float32 result."""
+    dt = _rows("x", x, dev_id)
+    n, dim = x.shape
+    wd = _operand("weight", weight, dev_id, 1, (dim,))[0]
+    for what, t in (("residual", residual), ("residual_out", residual_out)):
+        if t is not None and _rows(what, t, dev_id, (n, dim)) != dt:
+            raise LegionError("%s must be of x's type" % what)
+    if codec == CODEC_RAW:
+        if _rows("out", out, dev_id, (n, dim)) != dt:
+            raise LegionError("out must be of x's type")
+        stride = _row_stride(out)
+    else:
+        stride = _code_rows("out", out, dev_id, dim)
+        if out.shape[0] != n:
+            raise LegionError("out: %d rows, expected %d" % (out.shape[0], n))
+    _check(lib().legion_rms_norm(dev_id, x.data_ptr(), dt, _row_stride(x), None if residual is None else residual.data_ptr(),
+                                 0 if residual is None else _row_stride(residual), weight.data_ptr(), wd, eps, n, dim, codec,
+                                 out.data_ptr(), stride, None if residual_out is None else residual_out.data_ptr(),
+                                 0 if residual_out is None else _row_stride(residual_out), _handle(stream)))
+
+
+def rms_norm_grad_workspace(n_rows, dim):
+    """Bytes of scratch that rms_norm_grad takes."""
+    b = C.c_int64()
+    _check(lib().legion_rms_norm_grad_workspace(n_rows, dim, C.byref(b)))
+    return b.value
+
+
+def rms_norm_grad(dev_id, grad_out, x, weight, grad_x, grad_weight, workspace, eps=1e-6, grad_residual=None, stream=None):
+    """Gradients of rms_norm at the rows x that were normed (its residual_out, if it had a residual).  grad_residual: what reached
+    residual_out by other ways, added to grad_x."""
+    dt = _rows("x", x, dev_id)
+    n, dim = x.shape
+    for what, t in (("grad_out", grad_out), ("grad_x", grad_x), ("grad_residual", grad_residual)):
+        if (t is not None or what != "grad_residual") and _rows(what, t, dev_id, (n, dim)) != dt:
+            raise LegionError("%s must be of x's type" % what)
+    wd, gd = _operand("weight", weight, dev_id, 1, (dim,))[0], _operand("grad_weight", grad_weight, dev_id, 1, (dim,))[0]
+    ws, ws_bytes = _workspace(workspace, dev_id)
+    _check(lib().legion_rms_norm_grad(dev_id, grad_out.data_ptr(), _row_stride(grad_out), x.data_ptr(), _row_stride(x), dt,
+                                      None if grad_residual is None else grad_residual.data_ptr(),
+                                      0 if grad_residual is None else _row_stride(grad_residual), weight.data_ptr(), wd, eps, n, dim,
+                                      grad_x.data_ptr(), _row_stride(grad_x), grad_weight.data_ptr(), gd, ws, ws_bytes, _handle(stream)))
+
+
+def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None):
+    """out[i, j] = sum over the codes of row i and weight row j, times both rows' scales.  rows, weight_rows: uint8, compressed rows of
+    feature_len codes (rms_norm, quantize_table, a cache's partition); out: float32, float16 or bfloat16."""
+    rs, ws = _code_rows("rows", rows, dev_id, feature_len), _code_rows("weight_rows", weight_rows, dev_id, feature_len)
+    m, n = rows.shape[0], weight_rows.shape[0]
+    od = _rows("out", out, dev_id, (m, n))
+    _check(lib().legion_matmul_rows(dev_id, codec, rows.data_ptr(), m, rs, weight_rows.data_ptr(), n, ws, feature_len, out.data_ptr(), od,
+                                    _row_stride(out), _handle(stream)))
+
+
+def operator_error(dev_id, stream=None, reset=True):
+    """First error that a kernel of these operators raised on dev_id since the last reset (0: none)."""
+    e = C.c_int32()
+    _check(lib().legion_operator_error(dev_id, _handle(stream), C.byref(e), 1 if reset else 0))
+    return e.value
 
 
 class IPCEnv:

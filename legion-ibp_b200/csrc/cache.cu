@@ -6,11 +6,10 @@
 // StaticCache::init_cache (comp_cache/static_cache.cu:20-114).  The bucketed cuckoo table of
 // the reference (include/hashmap/bcht.hpp) becomes a direct table with one int32 per node:
 // one 4-byte read per lookup instead of up to three 128-byte bucket probes.
-#include "common.cuh"
+#include "codec.cuh"
 
 #include <cub/device/device_radix_sort.cuh>
 #include <cub/device/device_scan.cuh>
-#include <cuda_fp8.h>
 
 namespace legion {
 
@@ -119,31 +118,6 @@ static_fill_kernel(const int32_t *__restrict__ order, int64_t n_order, int32_t c
                 reinterpret_cast<uint32_t *>(dst)[q] = reinterpret_cast<const uint32_t *>(src)[q];
         }
     }
-}
-
-// Four codes of one row, first value in the low byte.  SAFE: any row; otherwise a row whose values and whose factor
-// are finite, where |x * inv| < 128 and the nearest integer is what adding 1.5 * 2^23 leaves in the low bits.
-template <int CODEC, bool SAFE>
-__device__ __forceinline__ uint32_t encode4(const float4 &x, float inv)
-{
-    const float p[4] = { __fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv) };
-    if (CODEC == LEGION_CODEC_INT8) {
-        uint32_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            q[i] = SAFE ? (uint32_t)max(-127, min(127, __float2int_rn(p[i]))) : __float_as_uint(__fadd_rn(p[i], 12582912.0f));
-        return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-    }
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p[0], p[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p[2], p[3]), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
-}
-
-__device__ __forceinline__ float max_nan(float a, float b)   // NaN when either is
-{
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
 }
 
 // Rows encoded: feature_len codes + one fp32 scale, zero padded to slot_bytes.  LPR lanes share a row, 32 / LPR rows

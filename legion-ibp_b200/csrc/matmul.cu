@@ -1,0 +1,495 @@
+// Products of compressed rows: out[i][j] = sa[i] * sb[j] * sum_k a[i][k] * b[j][k], codes int8 or e4m3, one fp32 scale per row
+// behind the codes.  Nothing is decoded: the codes go to the tensor cores as they lie in memory, the two scales
+// meet the sum in the epilogue.
+#include "codec.cuh"
+#include "typed.cuh"
+
+#include <cuda.h>
+#include <type_traits>
+
+namespace legion {
+
+static constexpr unsigned kFull = 0xFFFFFFFFu;
+
+__device__ int32_t g_operator_error = 0;
+
+// ---- PTX ---------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// About two seconds, then the wait is given up (false).
+constexpr long long kWaitClocks = 4000000000ll;
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity)
+{
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity))
+        if (clock64() - t0 > kWaitClocks) return false;
+    return true;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
+{
+    if (bar_try(bar, parity)) return true;
+    return bar_wait_long(bar, parity);
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+
+// Whether any of the 128 threads of warps 0 to 3 says so; a barrier among them.
+__device__ __forceinline__ bool any_of_128(bool mine)
+{
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(any) : "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
+
+// Shared-memory matrix descriptor of a K-major operand in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: D type (1 fp32, 2 int32) at bit 4, A and B types (int8: 1, e4m3: 0) at 7 and 10, N / 8 at 17, M / 16 at 24.
+template <int CODEC, int M, int N>
+__device__ __forceinline__ constexpr uint32_t instruction_desc()
+{
+    return (CODEC == LEGION_CODEC_INT8 ? (2u << 4 | 1u << 7 | 1u << 10) : 1u << 4) | (uint32_t)(N / 8) << 17 | (uint32_t)(M / 16) << 24;
+}
+template <int CODEC>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add)
+{
+    if (CODEC == LEGION_CODEC_INT8)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(idesc), "r"(add) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t *r);
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t addr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// ---- tensor-core kernel ----------------------------------------------------------------------------------------------
+
+struct MatmulParams {
+    const uint8_t *p_rows, *q_rows;   // the operand whose rows are TMEM lanes (tiles of 128), and the other
+    int64_t p_stride, q_stride;
+    int32_t p_n, q_n, k;
+    void *out;
+    int64_t out_stride;
+    int32_t out_dtype;
+};
+
+constexpr int kTileP = 128;
+constexpr int kTileK = 128;   // bytes of a row per stage: one swizzle line
+__host__ __device__ constexpr int stages_of(int bq) { return bq >= 256 ? 4 : (bq >= 128 ? 6 : 8); }
+__host__ __device__ constexpr int stage_bytes(int bq) { return (kTileP + bq) * kTileK; }
+__host__ __device__ constexpr int tmem_columns(int bq) { return 2 * bq < 32 ? 32 : 2 * bq; }
+constexpr int matmul_smem(int bq) { return stages_of(bq) * stage_bytes(bq) + 1024 + 2 * bq * 4 + 256; }
+
+// Tiles in groups of kGroupP along P, so that the tiles that run together share rows of both operands in L2.
+constexpr int kGroupP = 16;
+__device__ __forceinline__ void tile_at(int64_t t, int tiles_p, int tiles_q, int &p, int &q)
+{
+    const int64_t per_group = (int64_t)kGroupP * tiles_q;
+    const int g = (int)(t / per_group);
+    const int rest = (int)(t - g * per_group);
+    const int height = min(kGroupP, tiles_p - g * kGroupP);
+    q = rest / height;
+    p = g * kGroupP + rest - q * height;
+}
+
+// One CTA per SM takes tiles of 128 x BQ in turn.  Warp 4 loads stages of both operands by TMA, warp 5 issues the products into one of
+// two accumulators in TMEM, warps 0 to 3 scale and store the other one meanwhile.
+// P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.
+template <int CODEC, int BQ, bool P_OUT_COLUMNS>
+__global__ void __launch_bounds__(192, 1)
+matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map, MatmulParams m)
+{
+    constexpr int S = stages_of(BQ);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float *q_scale = reinterpret_cast<float *>(smem + S * stage_bytes(BQ));   // [2][BQ]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * BQ);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
+    volatile int32_t *gave_up = reinterpret_cast<volatile int32_t *>(tmem_slot + 1);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles_p = (m.p_n + kTileP - 1) / kTileP, tiles_q = (m.q_n + BQ - 1) / BQ;
+    const int64_t tiles = (int64_t)tiles_p * tiles_q;
+    const int blocks_k = (m.k + kTileK - 1) / kTileK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            bar_init(full + 8 * s, 1);
+            bar_init(empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            bar_init(acc_full + 8 * a, 1);
+            bar_init(acc_empty + 8 * a, 128);
+        }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            int64_t step = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                int tp, tq;
+                tile_at(t, tiles_p, tiles_q, tp, tq);
+                for (int kb = 0; kb < blocks_k; ++kb, ++step) {
+                    const int s = (int)(step % S);
+                    const uint32_t round = (uint32_t)(step / S);
+                    if (!bar_wait(empty + 8 * s, (round & 1) ^ 1) || *gave_up) { ok = false; break; }
+                    const uint32_t dst = smem_u32(smem + s * stage_bytes(BQ));
+                    bar_expect(full + 8 * s, stage_bytes(BQ));
+                    tma_2d(dst, &p_map, full + 8 * s, kb * kTileK, tp * kTileP);
+                    tma_2d(dst + kTileP * kTileK, &q_map, full + 8 * s, kb * kTileK, tq * BQ);
+                }
+            }
+            if (!ok) {  // the copies that are under way land before the CTA's memory goes
+                *gave_up = 1;
+                for (int64_t i = step > S ? step - S : 0; i < step; ++i) bar_wait(full + 8 * (int)(i % S), (uint32_t)(i / S) & 1);
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = instruction_desc<CODEC, kTileP, BQ>();
+            int64_t step = 0;
+            int turn = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++turn) {
+                const int a = turn & 1;
+                if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1) || *gave_up) { ok = false; break; }
+                fence_after();
+                for (int kb = 0; kb < blocks_k; ++kb, ++step) {
+                    const int s = (int)(step % S);
+                    if (!bar_wait(full + 8 * s, (uint32_t)(step / S) & 1) || *gave_up) { ok = false; break; }
+                    fence_after();
+                    const uint32_t src = smem_u32(smem + s * stage_bytes(BQ));
+                    const uint64_t dp = operand_desc(src), dq = operand_desc(src + kTileP * kTileK);
+                    // 32 codes a product; the last block has as many as the rows reach into
+                    const int products = min(kTileK / 32, (m.k - kb * kTileK + 31) / 32);
+                    for (int i = 0; i < products; ++i) mma<CODEC>(tmem + a * BQ, dp + 2 * i, dq + 2 * i, idesc, (kb | i) != 0);
+                    mma_commit(empty + 8 * s);
+                }
+                if (ok) mma_commit(acc_full + 8 * a);
+            }
+            if (!ok) *gave_up = 1;
+        }
+    } else {
+        int turn = 0;
+        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++turn) {
+            int tp, tq;
+            tile_at(t, tiles_p, tiles_q, tp, tq);
+            const int a = turn & 1;
+            const int p = tp * kTileP + warp * 32 + lane;
+            float *qs = q_scale + a * BQ;
+            for (int i = threadIdx.x; i < BQ; i += 128) {
+                const int q = tq * BQ + i;
+                qs[i] = q < m.q_n ? *reinterpret_cast<const float *>(m.q_rows + (int64_t)q * m.q_stride + m.k) : 0.0f;
+            }
+            const float ps = p < m.p_n ? *reinterpret_cast<const float *>(m.p_rows + (int64_t)p * m.p_stride + m.k) : 0.0f;
+            if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1)) *gave_up = 1;
+            if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < BQ; c += 16) {
+                uint32_t r[16];
+                tmem_load<16>(tmem + ((uint32_t)(warp * 32) << 16) + a * BQ + c, r);
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    v[i] = (CODEC == LEGION_CODEC_INT8 ? (float)(int32_t)r[i] : __uint_as_float(r[i])) * ps * qs[c + i];
+                const int q0 = tq * BQ + c;
+                if (p >= m.p_n || q0 >= m.q_n) continue;
+                if (P_OUT_COLUMNS) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (q0 + i < m.q_n) store_any(m.out, m.out_dtype, (int64_t)(q0 + i) * m.out_stride + p, v[i]);
+                } else {
+                    const int64_t at = (int64_t)p * m.out_stride + q0;
+                    uint8_t *dst = static_cast<uint8_t *>(m.out) + at * dtype_bytes(m.out_dtype);
+                    if (q0 + 16 <= m.q_n && (uintptr_t)dst % 16 == 0) {
+                        if (m.out_dtype == LEGION_F32) {
+                            Vec<float, 8> o[2];
+                            o[0].set(v); o[1].set(v + 8);
+                            o[0].store(reinterpret_cast<float *>(dst)); o[1].store(reinterpret_cast<float *>(dst) + 8);
+                        } else if (m.out_dtype == LEGION_F16) {
+                            Vec<__half, 8> o[2];
+                            o[0].set(v); o[1].set(v + 8);
+                            o[0].store(reinterpret_cast<__half *>(dst)); o[1].store(reinterpret_cast<__half *>(dst) + 8);
+                        } else {
+                            Vec<__nv_bfloat16, 8> o[2];
+                            o[0].set(v); o[1].set(v + 8);
+                            o[0].store(reinterpret_cast<__nv_bfloat16 *>(dst)); o[1].store(reinterpret_cast<__nv_bfloat16 *>(dst) + 8);
+                        }
+                    } else {
+                        for (int i = 0; i < 16 && q0 + i < m.q_n; ++i) store_any(m.out, m.out_dtype, at + i, v[i]);
+                    }
+                }
+            }
+            fence_before();
+            bar_arrive(acc_empty + 8 * a);
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (threadIdx.x == 0 && *gave_up) atomicCAS(&g_operator_error, 0, LEGION_E_TIMEOUT);
+    if (warp == 5) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_columns(BQ)));
+    }
+}
+
+// ---- few rows: no tiles ------------------------------------------------------------------------------------------------
+
+template <int CODEC>
+__device__ __forceinline__ void dot16(const uint4 &a, const uint4 &b, typename std::conditional<CODEC == LEGION_CODEC_INT8, int, float>::type &acc)
+{
+    const uint32_t x[4] = { a.x, a.y, a.z, a.w }, y[4] = { b.x, b.y, b.z, b.w };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (CODEC == LEGION_CODEC_INT8) {
+            acc = __dp4a((int)x[i], (int)y[i], acc);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const __half2_raw p = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x[i] >> (16 * h)), __NV_E4M3);
+                const __half2_raw q = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(y[i] >> (16 * h)), __NV_E4M3);
+                const float2 f = __half22float2(__half2(p)), g = __half22float2(__half2(q));
+                acc = fmaf(f.x, g.x, acc);
+                acc = fmaf(f.y, g.y, acc);
+            }
+        }
+    }
+}
+
+// A warp has R weight rows and all M rows of the other side: bound by the weights' bytes, each read once.
+template <int CODEC, int M, int R>
+__global__ void __launch_bounds__(256) matvec_kernel(MatmulParams m)
+{
+    typedef typename std::conditional<CODEC == LEGION_CODEC_INT8, int, float>::type acc_t;
+    const int lane = threadIdx.x & 31;
+    const int64_t n0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * R;
+    if (n0 >= m.p_n) return;
+    acc_t acc[R][M];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < M; ++i) acc[r][i] = 0;
+    const int chunks = m.k / 16;   // whole 16-byte pieces
+#pragma unroll 2
+    for (int c = lane; c < chunks; c += 32) {
+        uint4 w[R], x[M];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (n0 + r < m.p_n) w[r] = __ldcs(reinterpret_cast<const uint4 *>(m.p_rows + (n0 + r) * m.p_stride) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (i < m.q_n) x[i] = *(reinterpret_cast<const uint4 *>(m.q_rows + i * m.q_stride) + c);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < M; ++i) dot16<CODEC>(w[r], x[i], acc[r][i]);
+    }
+    const int rest = (m.k % 16) / 4;   // words behind them, one a lane
+    if (lane < rest) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (n0 + r >= m.p_n) continue;
+            const uint32_t w = reinterpret_cast<const uint32_t *>(m.p_rows + (n0 + r) * m.p_stride)[chunks * 4 + lane];
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+                if (i < m.q_n)
+                    dot16<CODEC>(make_uint4(w, 0, 0, 0),
+                                 make_uint4(reinterpret_cast<const uint32_t *>(m.q_rows + i * m.q_stride)[chunks * 4 + lane], 0, 0, 0), acc[r][i]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            acc_t a = acc[r][i];
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) a += __shfl_xor_sync(kFull, a, d);
+            if (lane == (r * M + i) % 32 && n0 + r < m.p_n && i < m.q_n) {
+                const float ws = *reinterpret_cast<const float *>(m.p_rows + (n0 + r) * m.p_stride + m.k);
+                const float xs = *reinterpret_cast<const float *>(m.q_rows + i * m.q_stride + m.k);
+                store_any(m.out, m.out_dtype, i * m.out_stride + n0 + r, (float)a * ws * xs);
+            }
+        }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled()
+{
+    static EncodeTiled fn = nullptr;
+    if (fn == nullptr) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiled)p;
+    }
+    return fn;
+}
+
+// k codes of n rows; what a box reaches beyond them (the scales among it) arrives as zeros
+static int make_map(CUtensorMap *map, const void *rows, int64_t n, int64_t stride, int32_t k, int box_rows)
+{
+    EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) {
+        set_error("legion_matmul_rows: the driver has no cuTensorMapEncodeTiled");
+        return LEGION_E_CUDA;
+    }
+    const cuuint64_t dims[2] = { (cuuint64_t)k, (cuuint64_t)n }, strides[1] = { (cuuint64_t)stride };
+    const cuuint32_t box[2] = { (cuuint32_t)kTileK, (cuuint32_t)box_rows }, one[2] = { 1, 1 };
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(rows), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("legion_matmul_rows: no tensor map for %lld rows of %d codes, %lld bytes apart (%d)", (long long)n, k, (long long)stride, (int)r);
+        return LEGION_E_CUDA;
+    }
+    return LEGION_OK;
+}
+
+template <int CODEC, int BQ, bool P_OUT_COLUMNS>
+static int launch_tiles(cudaStream_t s, const MatmulParams &m)
+{
+    CUtensorMap p_map, q_map;
+    int rc = make_map(&p_map, m.p_rows, m.p_n, m.p_stride, m.k, kTileP);
+    if (rc == LEGION_OK) rc = make_map(&q_map, m.q_rows, m.q_n, m.q_stride, m.k, BQ);
+    if (rc != LEGION_OK) return rc;
+    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, matmul_smem(BQ)));
+    const int64_t tiles = (int64_t)((m.p_n + kTileP - 1) / kTileP) * ((m.q_n + BQ - 1) / BQ);
+    matmul_kernel<CODEC, BQ, P_OUT_COLUMNS><<<(unsigned)(tiles < kSms ? tiles : kSms), 192, matmul_smem(BQ), s>>>(p_map, q_map, m);
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}
+
+template <int CODEC>
+static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t row_stride, const uint8_t *weights, int64_t n,
+                         int64_t weight_stride, int32_t k, void *out, int32_t out_dtype, int64_t out_stride)
+{
+    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype };
+    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype };
+    if (m <= 8) {
+#define LG_MATVEC(M, R) matvec_kernel<CODEC, M, R><<<(unsigned)((n + 8 * R - 1) / (8 * R)), 256, 0, s>>>(by_weight)
+        if (m == 1) LG_MATVEC(1, 2);
+        else if (m == 2) LG_MATVEC(2, 2);
+        else if (m <= 4) LG_MATVEC(4, 2);
+        else LG_MATVEC(8, 2);
+#undef LG_MATVEC
+        LG_LAUNCH_CHECK();
+        return LEGION_OK;
+    }
+    if (m <= 16) return launch_tiles<CODEC, 16, true>(s, by_weight);
+    if (m <= 32) return launch_tiles<CODEC, 32, true>(s, by_weight);
+    if (m <= 64) return launch_tiles<CODEC, 64, true>(s, by_weight);
+    if (m <= 128) return launch_tiles<CODEC, 128, true>(s, by_weight);
+    // wide tiles need the fewest bytes per product; narrower ones where they would leave SMs without work
+    const int64_t tiles_p = (m + kTileP - 1) / kTileP;
+    auto cost = [&](int bq) {
+        const int64_t tiles = tiles_p * ((n + bq - 1) / bq);
+        return (tiles + kSms - 1) / kSms * (bq + 96);
+    };
+    if (cost(256) <= cost(128) && cost(256) <= cost(64)) return launch_tiles<CODEC, 256, false>(s, by_row);
+    if (cost(128) <= cost(64)) return launch_tiles<CODEC, 128, false>(s, by_row);
+    return launch_tiles<CODEC, 64, false>(s, by_row);
+}
+
+}  // namespace legion
+
+using namespace legion;
+
+extern "C" int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t m, int64_t row_stride, const void *weight_rows,
+                                  int64_t n, int64_t weight_stride, int32_t feature_len, void *out, int32_t out_dtype, int64_t out_stride,
+                                  void *stream)
+{
+    LG_ARG(codec == LEGION_CODEC_INT8 || codec == LEGION_CODEC_E4M3, "codec must be INT8 or E4M3");
+    LG_ARG(feature_len > 0 && feature_len % 4 == 0, "compressed rows need feature_len % 4 == 0");
+    if (feature_len > LEGION_MATMUL_MAX_DIM) {
+        set_error("legion_matmul_rows: rows of %d codes are above the limit of %d", feature_len, LEGION_MATMUL_MAX_DIM);
+        return LEGION_E_LIMIT;
+    }
+    LG_ARG(m >= 0 && m < (1ll << 31) - 256 && n >= 0 && n < (1ll << 31) - 256, "m or n out of range");
+    LG_ARG(m == 0 || n == 0 || (rows != nullptr && weight_rows != nullptr && out != nullptr), "NULL pointer");
+    LG_ARG((uintptr_t)rows % 16 == 0 && (uintptr_t)weight_rows % 16 == 0, "compressed rows must start on multiples of 16 bytes");
+    LG_ARG(row_stride % 16 == 0 && row_stride >= code_row_bytes(feature_len) && row_stride < (1ll << 40) && weight_stride % 16 == 0 &&
+               weight_stride >= code_row_bytes(feature_len) && weight_stride < (1ll << 40),
+           "compressed rows are (feature_len + 4) rounded up to 16 bytes long, strides are multiples of 16 bytes");
+    LG_ARG(dtype_known(out_dtype), "out: dtype must be LEGION_F32, LEGION_F16 or LEGION_BF16");
+    LG_ARG(out_stride >= n && out_stride <= (1ll << 40) && (uintptr_t)out % dtype_bytes(out_dtype) == 0, "bad out stride or address");
+    if (m == 0 || n == 0) return LEGION_OK;
+    const OnDevice on(dev_id);
+    LG_CUDA(on.err);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (codec == LEGION_CODEC_INT8)
+        return launch_matmul<LEGION_CODEC_INT8>(s, (const uint8_t *)rows, m, row_stride, (const uint8_t *)weight_rows, n, weight_stride,
+                                                feature_len, out, out_dtype, out_stride);
+    return launch_matmul<LEGION_CODEC_E4M3>(s, (const uint8_t *)rows, m, row_stride, (const uint8_t *)weight_rows, n, weight_stride,
+                                            feature_len, out, out_dtype, out_stride);
+}
+
+extern "C" int legion_operator_error(int32_t dev_id, void *stream, int32_t *error, int32_t reset)
+{
+    LG_ARG(error != nullptr, "error is NULL");
+    const OnDevice on(dev_id);
+    LG_CUDA(on.err);
+    void *word = nullptr;
+    LG_CUDA(cudaGetSymbolAddress(&word, g_operator_error));
+    cudaStream_t s = (cudaStream_t)stream;
+    LG_CUDA(cudaMemcpyAsync(error, word, 4, cudaMemcpyDeviceToHost, s));
+    if (reset) LG_CUDA(cudaMemsetAsync(word, 0, 4, s));
+    LG_CUDA(cudaStreamSynchronize(s));
+    return LEGION_OK;
+}

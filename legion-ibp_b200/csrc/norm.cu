@@ -1,0 +1,489 @@
+// RMS norm with the residual's addition, its output as it is or as compressed rows, and its gradient.
+//
+//   h = x + r,   s = 1 / sqrt(mean(h^2) + eps),   y = h * w * s
+//   compressed: a = max |y|, scale = a / top, code = y * (top / a) rounded (the quantiser of the caches; top = 127 or 448)
+//   gradient, g = dy * w:   dx = s * g - h * s^3 * mean(g * h) (+ dres),   dw = sum over rows of dy * h * s
+//
+// A row is read once: a group of threads (8 or 32 lanes of a warp, or a CTA) holds it in registers from the loads through
+// the sums to the stores.  s is positive and rounding is monotone, so max |y| is s * max |h * w| to the bit, and the norm
+// and the codec share one reduction.  Sums are fp32, h is kept in fp32 until y is rounded; what
+// residual_out receives is h rounded once.  What bounds all of it is HBM.
+#include "codec.cuh"
+#include "typed.cuh"
+
+namespace legion {
+
+static constexpr unsigned kFull = 0xFFFFFFFFu;
+
+// Sum and, WITH_MAX, NaN-keeping maximum over the threads of a row.  GROUP lanes of a warp, or (0) the CTA.
+template <int GROUP>
+struct RowReduce {
+    float *smem;   // 2 x 2 x 32 words: two buffers used in turn, so that one barrier per row is enough
+    int flip = 0;
+    __device__ __forceinline__ explicit RowReduce(float *s) : smem(s) {}
+    __device__ __forceinline__ void two(float &a, float &b, bool second_is_max)
+    {
+        constexpr int kLanes = GROUP == 0 ? 32 : GROUP;
+#pragma unroll
+        for (int d = kLanes / 2; d > 0; d >>= 1) {
+            a += __shfl_xor_sync(kFull, a, d);
+            const float o = __shfl_xor_sync(kFull, b, d);
+            b = second_is_max ? max_nan(b, o) : b + o;
+        }
+        if (GROUP == 0) {
+            const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            float *sa = smem + flip * 64, *sb = sa + 32;
+            flip ^= 1;
+            if (lane == 0) {
+                sa[warp] = a;
+                sb[warp] = b;
+            }
+            __syncthreads();
+            a = lane < warps ? sa[lane] : 0.0f;
+            b = lane < warps ? sb[lane] : 0.0f;   // a maximum here is one of absolute values
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) {
+                a += __shfl_xor_sync(kFull, a, d);
+                const float o = __shfl_xor_sync(kFull, b, d);
+                b = second_is_max ? max_nan(b, o) : b + o;
+            }
+        }
+    }
+};
+
+struct NormParams {
+    const void *x, *residual, *weight;
+    void *out, *residual_out;
+    int64_t n, x_stride, residual_stride, out_stride, residual_out_stride;  // out_stride: bytes for compressed rows
+    int32_t dim, weight_dtype;
+    float eps;
+};
+
+template <int VE>
+__device__ __forceinline__ void store_codes(uint8_t *p, const uint32_t *c)
+{
+    if (VE == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(c[0], c[1 % ((VE + 3) / 4)]);
+    else if (VE == 4) *reinterpret_cast<uint32_t *>(p) = c[0];
+    else if (VE == 2) *reinterpret_cast<uint16_t *>(p) = (uint16_t)c[0];
+    else *p = (uint8_t)c[0];
+}
+
+template <typename T, int VE, int U, int GROUP, int CODEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
+{
+    __shared__ float smem[128];
+    RowReduce<GROUP> reduce(smem);
+    const int width = GROUP == 0 ? blockDim.x : GROUP;
+    const int t = GROUP == 0 ? threadIdx.x : threadIdx.x & (GROUP - 1);
+    const int per_cta = GROUP == 0 ? 1 : 128 / (GROUP == 0 ? 1 : GROUP);
+    float w[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int col = (t + u * width) * VE;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[u][i] = col < p.dim ? load_any(p.weight, p.weight_dtype, col + i) : 0.0f;
+    }
+    const float top = CODEC == LEGION_CODEC_INT8 ? 127.0f : 448.0f;
+    // the rows of a CTA's groups end together, so that every lane takes part in the reductions
+    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += (int64_t)gridDim.x * per_cta) {
+        const int64_t row = row0 + (GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP));
+        const bool in = row < p.n;
+        float h[U][VE];
+        float sum = 0.0f, most = 0.0f;
+        {
+            Vec<T, VE> a[U], r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int col = (t + u * width) * VE;
+                a[u].zero();
+                if (in && col < p.dim) a[u].load(static_cast<const T *>(p.x) + row * p.x_stride + col);
+                if (p.residual != nullptr) {
+                    r[u].zero();
+                    if (in && col < p.dim) r[u].load(static_cast<const T *>(p.residual) + row * p.residual_stride + col);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int col = (t + u * width) * VE;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    h[u][i] = a[u].get(i);
+                    if (p.residual != nullptr) h[u][i] += r[u].get(i);
+                    sum = fmaf(h[u][i], h[u][i], sum);
+                }
+                if (p.residual_out != nullptr && in && col < p.dim) {
+                    Vec<T, VE> o;
+                    o.set(h[u]);
+                    o.store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride + col);
+                }
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    h[u][i] *= w[u][i];
+                    if (CODEC != LEGION_CODEC_RAW && col < p.dim) most = max_nan(most, fabsf(h[u][i]));
+                }
+            }
+        }
+        reduce.two(sum, most, true);
+        const float s = 1.0f / sqrtf(sum / (float)p.dim + p.eps);
+        if (CODEC == LEGION_CODEC_RAW) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int col = (t + u * width) * VE;
+                if (!in || col >= p.dim) continue;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) h[u][i] *= s;
+                Vec<T, VE> o;
+                o.set(h[u]);
+                o.store(static_cast<T *>(p.out) + row * p.out_stride + col);
+            }
+            continue;
+        }
+        most *= s;
+        const bool plain_max = __float_as_uint(most) < 0x7F800000u;
+        if (GROUP == 0 ? !plain_max : __any_sync(kFull, !plain_max)) {
+            // not all values are numbers: the scale is that of those that are
+            float num = 0.0f, unused = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if ((t + u * width) * VE < p.dim) num = fmaxf(num, fabsf(h[u][i] * s));
+            reduce.two(unused, num, true);
+            if (!plain_max) most = num;
+        }
+        const float inv = most > 0.0f ? __fdiv_rn(top, most) : 0.0f, scale = __fdiv_rn(most, top);
+        const bool plain = plain_max && __float_as_uint(inv) < 0x7F800000u;
+        if (!in) continue;
+        uint8_t *dst = static_cast<uint8_t *>(p.out) + row * p.out_stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            if (col >= p.dim) continue;
+            uint32_t c[(VE + 3) / 4];
+#pragma unroll
+            for (int q = 0; q < (VE + 3) / 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = 4 * q + i < VE ? h[u][(4 * q + i) % VE] * s : 0.0f;
+                const float4 f = make_float4(v[0], v[1], v[2], v[3]);
+                c[q] = plain ? encode4<CODEC, false>(f, inv) : encode4<CODEC, true>(f, inv);
+            }
+            store_codes<VE>(dst + col, c);
+        }
+        const int tail = (int)((code_row_bytes(p.dim) - p.dim) >> 2);
+        if (t < tail) reinterpret_cast<uint32_t *>(dst + p.dim)[t] = t == 0 ? __float_as_uint(scale) : 0u;
+    }
+}
+
+struct NormGradParams {
+    const void *grad_out, *x, *grad_residual, *weight;
+    void *grad_x;
+    float *part;   // [CTA][dim]: the CTA's rows' share of the weight's gradient
+    int64_t n, grad_stride, x_stride, grad_residual_stride, grad_x_stride;
+    int32_t dim, weight_dtype;
+    float eps;
+};
+
+template <typename T, int VE, int U, int GROUP, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
+{
+    __shared__ float smem[128];
+    __shared__ float cross[GROUP == 0 ? 1 : 128 * U * VE];
+    RowReduce<GROUP> reduce(smem);
+    const int width = GROUP == 0 ? blockDim.x : GROUP;
+    const int t = GROUP == 0 ? threadIdx.x : threadIdx.x & (GROUP - 1);
+    const int per_cta = GROUP == 0 ? 1 : 128 / (GROUP == 0 ? 1 : GROUP);
+    float w[U][VE], dw[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int col = (t + u * width) * VE;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            w[u][i] = col < p.dim ? load_any(p.weight, p.weight_dtype, col + i) : 0.0f;
+            dw[u][i] = 0.0f;
+        }
+    }
+    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += (int64_t)gridDim.x * per_cta) {
+        const int64_t row = row0 + (GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP));
+        const bool in = row < p.n;
+        Vec<T, VE> h[U], dy[U], r[U];
+        float square = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            h[u].zero();
+            dy[u].zero();
+            if (p.grad_residual != nullptr) r[u].zero();
+            if (in && col < p.dim) {
+                h[u].load_stream(static_cast<const T *>(p.x) + row * p.x_stride + col);
+                dy[u].load_stream(static_cast<const T *>(p.grad_out) + row * p.grad_stride + col);
+                if (p.grad_residual != nullptr)
+                    r[u].load(static_cast<const T *>(p.grad_residual) + row * p.grad_residual_stride + col);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float a = h[u].get(i);
+                square = fmaf(a, a, square);
+                dot = fmaf(dy[u].get(i) * w[u][i], a, dot);
+            }
+        reduce.two(square, dot, false);
+        const float s = 1.0f / sqrtf(square / (float)p.dim + p.eps);
+        const float k = s * s * s * (dot / (float)p.dim);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            if (!in || col >= p.dim) continue;
+            float dx[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float a = h[u].get(i), g = dy[u].get(i);
+                dx[i] = s * (g * w[u][i]) - a * k;
+                if (p.grad_residual != nullptr) dx[i] += r[u].get(i);
+                dw[u][i] = fmaf(g, a * s, dw[u][i]);
+            }
+            Vec<T, VE> o;
+            o.set(dx);
+            o.store(static_cast<T *>(p.grad_x) + row * p.grad_x_stride + col);
+        }
+    }
+    float *part = p.part + (int64_t)blockIdx.x * p.dim;
+    if (GROUP == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if ((t + u * width) * VE < p.dim) part[(t + u * width) * VE + i] = dw[u][i];
+        return;
+    }
+    // the groups of a CTA add theirs in group order
+    constexpr int kCols = (GROUP == 0 ? 1 : GROUP) * U * VE;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) cross[(threadIdx.x / (GROUP == 0 ? 1 : GROUP)) * kCols + (t + u * GROUP) * VE + i] = dw[u][i];
+    __syncthreads();
+    for (int col = threadIdx.x; col < p.dim; col += 128) {
+        float sum = 0.0f;
+        for (int g = 0; g < per_cta; ++g) sum += cross[g * kCols + col];
+        part[col] = sum;
+    }
+}
+
+// Columns of the CTAs' shares added: 32 columns a CTA, 32 threads a column, one fixed order.
+__global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float *__restrict__ part, int parts, int dim, void *out, int dtype)
+{
+    __shared__ float s[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + x;
+    float sum = 0.0f;
+    if (col < dim)
+#pragma unroll 4
+        for (int g = y; g < parts; g += 32) sum += part[(int64_t)g * dim + col];
+    s[y][x] = sum;
+    __syncthreads();
+    sum = s[x][y];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+    if (x == 0 && blockIdx.x * 32 + y < dim) store_any(out, dtype, blockIdx.x * 32 + y, sum);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------
+
+constexpr int kGradCtas = 4 * kSms;  // most CTAs of the gradient: their shares of the weight's gradient lie in scratch
+
+// How a row of `vecs` vectors is held: lanes of a warp as long as four vectors a lane hold it, a CTA behind that.
+struct RowShape {
+    int group, u, threads, per_cta;
+};
+static RowShape row_shape(int vecs, int64_t n)
+{
+    if (vecs <= 8) return { 8, 1, 128, 16 };
+    if (vecs <= 32) return { 32, 1, 128, 4 };
+    if (vecs <= 64) return { 32, 2, 128, 4 };
+    int u = 1;  // few rows: as many threads as there are vectors; many: CTAs of about 256 threads, so that several are on an SM
+    if (n >= 2 * kSms)
+        while (u < 4 && (vecs + u - 1) / u > 256) u *= 2;
+    while ((vecs + u - 1) / u > 1024) u *= 2;
+    return { 0, u, ((vecs + u - 1) / u + 31) / 32 * 32, 1 };
+}
+
+template <typename T, int VE, int CODEC>
+static int launch_norm(cudaStream_t s, const NormParams &p)
+{
+    const RowShape r = row_shape(p.dim / VE, p.n);
+    const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
+    const int64_t most = (int64_t)kSms * (2048 / r.threads);
+    const unsigned grid = (unsigned)(need < most ? need : most);
+#define LG_NORM(U, GROUP, MAXT) norm_kernel<T, VE, U, GROUP, CODEC, MAXT><<<grid, r.threads, 0, s>>>(p)
+// registers are what a CTA of 1024 threads lacks: rows that smaller CTAs hold get kernels with more of them
+#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, (U * VE > 16 ? 512 : 1024)); } while (0)
+    if (r.group == 8) LG_NORM(1, 8, 128);
+    else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
+    else if (r.u == 1) LG_NORM_CTA(1);
+    else if (r.u == 2) LG_NORM_CTA(2);
+    else if (r.u == 4) LG_NORM_CTA(4);
+    else if (r.u == 8) { if constexpr (VE <= 2) LG_NORM(8, 0, 1024); }
+    else { if constexpr (VE == 1) LG_NORM(16, 0, 1024); }
+#undef LG_NORM_CTA
+#undef LG_NORM
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}
+
+template <typename T, int CODEC>
+static int launch_norm_ve(cudaStream_t s, const NormParams &p, int ve)
+{
+    switch (ve) {
+    case 8:
+        if constexpr (sizeof(T) == 2) return launch_norm<T, 8, CODEC>(s, p);
+    case 4: return launch_norm<T, 4, CODEC>(s, p);
+    case 2: return launch_norm<T, 2, CODEC>(s, p);
+    default: return launch_norm<T, 1, CODEC>(s, p);
+    }
+}
+
+template <typename T>
+static int launch_norm_codec(cudaStream_t s, const NormParams &p, int codec, int ve)
+{
+    if (codec == LEGION_CODEC_RAW) return launch_norm_ve<T, LEGION_CODEC_RAW>(s, p, ve);
+    if (codec == LEGION_CODEC_INT8) return launch_norm_ve<T, LEGION_CODEC_INT8>(s, p, ve);
+    return launch_norm_ve<T, LEGION_CODEC_E4M3>(s, p, ve);
+}
+
+template <typename T, int VE>
+static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
+{
+    const RowShape r = row_shape(p.dim / VE, p.n);
+    const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
+    const unsigned grid = (unsigned)(need < kGradCtas ? need : kGradCtas);
+    *parts = (int)grid;
+#define LG_NORM(U, GROUP, MAXT) norm_grad_kernel<T, VE, U, GROUP, MAXT><<<grid, r.threads, 0, s>>>(p)
+// registers are what a CTA of 1024 threads lacks: rows that smaller CTAs hold get kernels with more of them
+#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, (U * VE > 16 ? 512 : 1024)); } while (0)
+    if (r.group == 8) LG_NORM(1, 8, 128);
+    else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
+    else if (r.u == 1) LG_NORM_CTA(1);
+    else if (r.u == 2) LG_NORM_CTA(2);
+    else if (r.u == 4) LG_NORM_CTA(4);
+    else if (r.u == 8) { if constexpr (VE <= 2) LG_NORM(8, 0, 1024); }
+    else { if constexpr (VE == 1) LG_NORM(16, 0, 1024); }
+#undef LG_NORM_CTA
+#undef LG_NORM
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}
+
+template <typename T>
+static int launch_norm_grad_ve(cudaStream_t s, const NormGradParams &p, int ve, int *parts)
+{
+    switch (ve) {
+    case 8:
+        if constexpr (sizeof(T) == 2) return launch_norm_grad<T, 8>(s, p, parts);
+    case 4: return launch_norm_grad<T, 4>(s, p, parts);
+    case 2: return launch_norm_grad<T, 2>(s, p, parts);
+    default: return launch_norm_grad<T, 1>(s, p, parts);
+    }
+}
+
+}  // namespace legion
+
+using namespace legion;
+
+// a row operand of the call's type: NULL only where it may be
+#define LG_OPERAND(p, stride, dim, dtype, what)                                                          \
+    LG_ARG((uintptr_t)(p) % dtype_bytes(dtype) == 0, what " must start on a multiple of its element's size"); \
+    LG_ARG((p) == nullptr || ((stride) >= (dim) && (stride) <= (1ll << 40)), what ": a row's stride must be at least its length")
+
+extern "C" int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stride, const void *residual,
+                               int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim,
+                               int32_t codec, void *out, int64_t out_stride, void *residual_out, int64_t residual_out_stride, void *stream)
+{
+    LG_ARG(dtype_known(dtype), "dtype must be LEGION_F32, LEGION_F16 or LEGION_BF16");
+    LG_ARG(weight_dtype == dtype || weight_dtype == LEGION_F32, "weight must be fp32 or of the rows' type");
+    LG_ARG(codec >= LEGION_CODEC_RAW && codec <= LEGION_CODEC_E4M3, "codec must be RAW, INT8 or E4M3");
+    LG_ARG(dim > 0 && dim <= LEGION_NORM_MAX_DIM, "dim out of range");
+    LG_ARG(codec == LEGION_CODEC_RAW || dim % 4 == 0, "compressed rows need dim % 4 == 0");
+    LG_ARG(n_rows >= 0 && n_rows < (1ll << 31), "n_rows out of range");
+    LG_ARG(eps >= 0.0f, "eps must not be negative");
+    LG_ARG(n_rows == 0 || (x != nullptr && out != nullptr && weight != nullptr), "NULL pointer");
+    LG_ARG((uintptr_t)weight % dtype_bytes(weight_dtype) == 0, "weight must start on a multiple of its element's size");
+    LG_OPERAND(x, x_stride, dim, dtype, "x");
+    LG_OPERAND(residual, residual_stride, dim, dtype, "residual");
+    LG_OPERAND(residual_out, residual_out_stride, dim, dtype, "residual_out");
+    if (codec == LEGION_CODEC_RAW) {
+        LG_OPERAND(out, out_stride, dim, dtype, "out");
+    } else {
+        LG_ARG((uintptr_t)out % 16 == 0 && out_stride % 16 == 0 && out_stride >= code_row_bytes(dim),
+               "compressed rows start on multiples of 16 bytes and are (dim + 4) rounded up to 16 bytes long");
+    }
+    if (n_rows == 0) return LEGION_OK;
+    const OnDevice on(dev_id);
+    LG_CUDA(on.err);
+    NormParams p{ x, residual, weight, out, residual_out, n_rows, x_stride, residual_stride, out_stride, residual_out_stride, dim,
+                  weight_dtype, eps };
+    int ve = common_vector(dtype == LEGION_F32 ? 4 : 8, { dim, x_stride, aligned_elements(x, dtype) });
+    if (residual != nullptr) ve = common_vector(ve, { residual_stride, aligned_elements(residual, dtype) });
+    if (residual_out != nullptr) ve = common_vector(ve, { residual_out_stride, aligned_elements(residual_out, dtype) });
+    if (codec == LEGION_CODEC_RAW) ve = common_vector(ve, { out_stride, aligned_elements(out, dtype) });
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == LEGION_F32) return launch_norm_codec<float>(s, p, codec, ve);
+    if (dtype == LEGION_F16) return launch_norm_codec<__half>(s, p, codec, ve);
+    return launch_norm_codec<__nv_bfloat16>(s, p, codec, ve);
+}
+
+static int64_t norm_grad_scratch(int64_t n_rows, int32_t dim) { return (n_rows < kGradCtas ? n_rows : kGradCtas) * (int64_t)dim * 4; }
+
+extern "C" int legion_rms_norm_grad_workspace(int64_t n_rows, int32_t dim, int64_t *bytes)
+{
+    LG_ARG(bytes != nullptr, "bytes is NULL");
+    LG_ARG(dim > 0 && dim <= LEGION_NORM_MAX_DIM, "dim out of range");
+    LG_ARG(n_rows >= 0 && n_rows < (1ll << 31), "n_rows out of range");
+    *bytes = norm_grad_scratch(n_rows, dim);
+    return LEGION_OK;
+}
+
+extern "C" int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_t grad_stride, const void *x, int64_t x_stride,
+                                    int32_t dtype, const void *grad_residual, int64_t grad_residual_stride, const void *weight,
+                                    int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim, void *grad_x, int64_t grad_x_stride,
+                                    void *grad_weight, int32_t grad_weight_dtype, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    LG_ARG(dtype_known(dtype), "dtype must be LEGION_F32, LEGION_F16 or LEGION_BF16");
+    LG_ARG(weight_dtype == dtype || weight_dtype == LEGION_F32, "weight must be fp32 or of the rows' type");
+    LG_ARG(grad_weight_dtype == dtype || grad_weight_dtype == LEGION_F32, "grad_weight must be fp32 or of the rows' type");
+    LG_ARG(dim > 0 && dim <= LEGION_NORM_MAX_DIM, "dim out of range");
+    LG_ARG(n_rows >= 0 && n_rows < (1ll << 31), "n_rows out of range");
+    LG_ARG(eps >= 0.0f, "eps must not be negative");
+    LG_ARG(grad_weight != nullptr && weight != nullptr, "NULL pointer");
+    LG_ARG(n_rows == 0 || (x != nullptr && grad_out != nullptr && grad_x != nullptr), "NULL pointer");
+    LG_ARG((uintptr_t)weight % dtype_bytes(weight_dtype) == 0, "weight must start on a multiple of its element's size");
+    LG_ARG((uintptr_t)grad_weight % dtype_bytes(grad_weight_dtype) == 0, "grad_weight must start on a multiple of its element's size");
+    LG_OPERAND(x, x_stride, dim, dtype, "x");
+    LG_OPERAND(grad_out, grad_stride, dim, dtype, "grad_out");
+    LG_OPERAND(grad_x, grad_x_stride, dim, dtype, "grad_x");
+    LG_OPERAND(grad_residual, grad_residual_stride, dim, dtype, "grad_residual");
+    LG_ARG(n_rows == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace is NULL or not on a multiple of 16 bytes");
+    LG_ARG(workspace_bytes >= norm_grad_scratch(n_rows, dim), "workspace is smaller than the call asks for");
+    const OnDevice on(dev_id);
+    LG_CUDA(on.err);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (n_rows == 0) {
+        LG_CUDA(cudaMemsetAsync(grad_weight, 0, (size_t)dim * dtype_bytes(grad_weight_dtype), s));
+        return LEGION_OK;
+    }
+    NormGradParams p{ grad_out, x, grad_residual, weight, grad_x, (float *)workspace, n_rows, grad_stride, x_stride, grad_residual_stride,
+                      grad_x_stride, dim, weight_dtype, eps };
+    int ve = common_vector(dtype == LEGION_F32 ? 4 : 8, { dim, x_stride, aligned_elements(x, dtype), grad_stride, aligned_elements(grad_out, dtype),
+                                                          grad_x_stride, aligned_elements(grad_x, dtype) });
+    if (grad_residual != nullptr) ve = common_vector(ve, { grad_residual_stride, aligned_elements(grad_residual, dtype) });
+    int parts = 0, rc;
+    if (dtype == LEGION_F32) rc = launch_norm_grad_ve<float>(s, p, ve, &parts);
+    else if (dtype == LEGION_F16) rc = launch_norm_grad_ve<__half>(s, p, ve, &parts);
+    else rc = launch_norm_grad_ve<__nv_bfloat16>(s, p, ve, &parts);
+    if (rc != LEGION_OK) return rc;
+    norm_weight_grad_kernel<<<(dim + 31) / 32, 1024, 0, s>>>((const float *)workspace, parts, dim, grad_weight, grad_weight_dtype);
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}

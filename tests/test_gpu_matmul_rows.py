@@ -1,0 +1,191 @@
+"""Products of compressed rows against 64-bit sums over the codes.
+
+Tolerances: int8 sums are exact; the sum becomes fp32 and meets two scales, three roundings of 2^-24, then one of the output's
+type.  e4m3: products of two codes are exact in fp32, K of them are added with at most one step (2^-23) lost per
+addition, relative to the sum of their magnitudes."""
+import numpy as np
+import pytest
+
+import legion_ibp_b200 as L
+from test_gpu_embedding import U32, _close, _strided, _types
+
+pytestmark = pytest.mark.gpu
+CODECS = [L.CODEC_INT8, L.CODEC_E4M3]
+
+
+def _coded(n, k, codec, pad=0, seed=0, std=1.0):
+    """Compressed rows (random codes of a normal distribution, one scale a row), bytes behind the scale filled with 0xFF."""
+    import torch
+    torch.manual_seed(seed + 7 * n + k)
+    slot = (k + 19) // 16 * 16 + pad
+    rows = torch.full((n, slot), 0xFF, dtype=torch.uint8, device="cuda")
+    x = torch.randn(n, k, device="cuda") * std
+    codes = (x * 40).round().clamp(-128, 127).to(torch.int8) if codec == L.CODEC_INT8 else (x * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    rows[:, :k] = codes.view(torch.uint8)
+    scale = torch.exp(torch.randn(n, device="cuda"))
+    rows.view(torch.float32)[:, k // 4] = scale
+    return rows, codes.double(), scale.double()
+
+
+def _check(got, a, b, k, codec):
+    (_, ca, sa), (_, cb, sb) = a, b
+    outer = sa[:, None] * sb[None]
+    want = (ca @ cb.t()) * outer
+    slack = want.abs() * (3 * U32)
+    if codec == L.CODEC_E4M3:
+        slack = slack + (ca.abs() @ cb.abs().t()) * outer * (k * 2 * U32)
+    _close(got, want, slack)
+
+
+SHAPES = [(1, 1, 4), (1, 5, 16), (2, 33, 20), (3, 130, 36), (4, 64, 128), (5, 1000, 132), (7, 16, 2048), (8, 17, 1028), (9, 300, 64), (16, 128, 256),
+          (17, 129, 260), (33, 500, 768), (64, 64, 516), (65, 257, 100), (127, 128, 128), (128, 1000, 384), (129, 100, 132), (200, 513, 1024),
+          (300, 256, 640), (611, 1000, 768), (1030, 70, 40), (257, 2600, 4096), (5000, 260, 128)]
+
+
+@pytest.mark.parametrize("codec", CODECS)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("out_type", ["f32", "f16", "bf16"])
+def test_product(codec, m, n, k, out_type):
+    import torch
+    t = _types()[out_type]
+    for pad, out_pad, shift in ((0, 0, 0), (32, 3, 1)):
+        a, b = _coded(m, k, codec, pad, 1), _coded(n, k, codec, pad, 2, 0.3 if out_type == "f16" else 1.0)
+        if out_type == "f16":   # inside the range of the type
+            a = (a[0], a[1], a[2] / 4096)
+            a[0].view(torch.float32)[:, k // 4] = a[2].float()
+        whole, out = _strided(m, n, t, out_pad, shift)
+        L.matmul_rows(0, codec, a[0], b[0], k, out)
+        _check(out, a, b, k, codec)
+        rest = whole.clone()
+        torch.as_strided(rest, (m, n), (n + out_pad, 1), shift).fill_(7.0)
+        assert bool((rest == 7.0).all())
+        assert L.operator_error(0) == 0
+
+
+@pytest.mark.parametrize("m", [1, 9, 40, 300])
+def test_int8_sums_are_exact_at_their_limits(m):
+    """The longest rows, all codes -128 on both sides: the sum is 128 * 128 * K, close below 2^31."""
+    import torch
+    k = 131068
+    rows = torch.zeros(m, k + 4, dtype=torch.uint8, device="cuda")
+    rows[:, :k] = 128
+    rows.view(torch.float32)[:, k // 4] = 1.0
+    out = torch.zeros(m, m, device="cuda")
+    L.matmul_rows(0, L.CODEC_INT8, rows, rows, k, out)
+    assert bool((out == float(np.float32(128 * 128 * k))).all())
+
+
+@pytest.mark.parametrize("codec", CODECS)
+@pytest.mark.parametrize("m", [3, 20, 200])
+def test_scales_of_zero_infinity_and_nan_stay_in_their_row(codec, m):
+    import torch
+    a, b = _coded(m, 64, codec, 0, 3), _coded(40, 64, codec, 0, 4)
+    a[0].view(torch.float32)[1, 16] = 0.0
+    b[0].view(torch.float32)[2, 16] = float("nan")
+    out = torch.empty(m, 40, device="cuda")
+    L.matmul_rows(0, codec, a[0], b[0], 64, out)
+    bad = torch.isnan(out)
+    assert bool(bad[:, 2].all()) and int(bad.sum()) == m
+    assert bool((out[1].nan_to_num(0.0) == 0).all())
+
+
+def test_rows_of_a_cache_partition(oracle_mod):
+    """A compressed cache's partition is projected as it lies in memory: what decoding and multiplying gives."""
+    import torch
+    rng = np.random.default_rng(5)
+    n, f, h = 900, 100, 48
+    table = rng.standard_normal((n, f)).astype(np.float32)
+    for codec in CODECS:
+        cache = L.UnifiedCache(0, n, f * 4, n, codec=codec)
+        order = torch.from_numpy(rng.permutation(n).astype(np.int32)).cuda()
+        cache.fill_static(order, torch.from_numpy(table).pin_memory())
+        torch.cuda.synchronize()
+        weight = torch.randn(h, f, device="cuda")
+        coded = torch.empty(h, oracle_mod.quant_row_bytes(f), dtype=torch.uint8, device="cuda")
+        L.quantize_table(0, codec, weight, h, f, coded)
+        stored = oracle_mod.quant_rows(table[order.cpu().numpy()], codec)
+        ptr, nbytes = cache.partition()
+        assert nbytes == stored.size
+        rows = torch.empty(n, stored.shape[1], dtype=torch.uint8, device="cuda")
+        L._check(L.lib().legion_copy(L._ptr(rows), L.C.c_void_p(ptr), L.C.c_int64(nbytes), L.C.c_int32(3)))
+        out = torch.empty(n, h, device="cuda")
+        L.matmul_rows(0, codec, rows, coded, f, out)
+        a = oracle_mod.dequant_rows(stored, f, codec).astype(np.float64)
+        b = oracle_mod.dequant_rows(coded.cpu().numpy(), f, codec).astype(np.float64)
+        # decoding rounds each value once more (2^-24 of it)
+        slack = (np.abs(a) @ np.abs(b).T) * ((2 * f + 8) * U32)
+        assert (np.abs(out.cpu().numpy().astype(np.float64) - a @ b.T) <= slack + np.abs(a @ b.T) * U32).all()
+        cache.close()
+
+
+@pytest.mark.parametrize("codec", CODECS)
+def test_lookup_norm_product_and_back(codec):
+    """A run as it is used: learned rows, norm to compressed rows, product; the way back through norm and lookup."""
+    import torch
+    torch.manual_seed(2)
+    n, nodes, dim, width = 777, 400, 256, 130
+    table, w, weight = torch.randn(nodes, dim, device="cuda"), 1 + 0.1 * torch.randn(dim, device="cuda"), torch.randn(width, dim, device="cuda")
+    ids = torch.randint(0, nodes, (n,), device="cuda", dtype=torch.int32)
+    slot = (dim + 19) // 16 * 16
+    coded_w = torch.empty(width, slot, dtype=torch.uint8, device="cuda")
+    L.quantize_table(0, codec, weight, width, dim, coded_w)
+    x, coded, out = torch.empty(n, dim, device="cuda"), torch.empty(n, slot, dtype=torch.uint8, device="cuda"), torch.empty(n, width, device="cuda")
+    L.embedding_lookup(0, table, ids, x, 2.0)
+    L.rms_norm(0, x, w, coded, 1e-6, codec=codec)
+    L.matmul_rows(0, codec, coded, coded_w, dim, out)
+    h = table.double()[ids.long()] * 2
+    y = h * w.double() / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6)
+    want = y @ weight.double().t()
+    # both sides are off by half a step of their codes: int8 half of max / 127 each; e4m3 2^-4 of the value, or 2^-10 of max / 448
+    if codec == L.CODEC_INT8:
+        ey, ew = y.abs().amax(1, keepdim=True) / 254, weight.double().abs().amax(1, keepdim=True) / 254
+        slack = ey * weight.double().abs().sum(1)[None] + y.abs().sum(1, keepdim=True) * ew.t() + dim * ey * ew.t()
+    else:
+        ey = y.abs() * 2 ** -4 + y.abs().amax(1, keepdim=True) / 448 * 2 ** -10
+        ew = weight.double().abs() * 2 ** -4 + weight.double().abs().amax(1, keepdim=True) / 448 * 2 ** -10
+        slack = ey @ weight.double().abs().t() + y.abs() @ ew.t() + ey @ ew.t()
+    assert bool(((out.double() - want).abs() <= slack * 1.001 + 1e-4).all())
+    dy, dx, dw, grad = torch.randn(n, dim, device="cuda"), torch.empty(n, dim, device="cuda"), torch.empty(dim, device="cuda"), torch.empty(nodes, dim, device="cuda")
+    L.rms_norm_grad(0, dy, x, w, dx, dw, torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda"))
+    L.embedding_grad(0, ids, dx, grad, torch.empty(L.embedding_grad_workspace(n, dim, nodes), dtype=torch.uint8, device="cuda"), 2.0)
+    leaf = table.double().requires_grad_()
+    hh = leaf[ids.long()] * 2
+    ((hh * w.double() / torch.sqrt((hh * hh).mean(1, keepdim=True) + 1e-6)) * dy.double()).sum().backward()
+    assert float((grad.double() - leaf.grad).abs().max()) <= 1e-4 * float(leaf.grad.abs().max())
+
+
+def test_captured_with_other_rows():
+    import torch
+    for m in (2, 24, 300):
+        a, b = _coded(m, 256, L.CODEC_INT8, 0, 5), _coded(200, 256, L.CODEC_INT8, 0, 6)
+        out = torch.empty(m, 200, device="cuda")
+        side = torch.cuda.Stream()
+        L.matmul_rows(0, L.CODEC_INT8, a[0], b[0], 256, out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            L.matmul_rows(0, L.CODEC_INT8, a[0], b[0], 256, out, stream=torch.cuda.current_stream())
+        c = _coded(m, 256, L.CODEC_INT8, 0, 9)
+        a[0].copy_(c[0])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        _check(out, c, b, 256, L.CODEC_INT8)
+
+
+def test_nothing_to_do_and_refusals():
+    import torch
+    a, b = _coded(4, 64, 1)[0], _coded(6, 64, 1)[0]
+    out = torch.full((4, 6), 3.0, device="cuda")
+    L.matmul_rows(0, 1, a[:0], b, 64, out[:0])
+    for bad in (lambda: L.matmul_rows(0, 0, a, b, 64, out), lambda: L.matmul_rows(0, 1, a, b, 62, out), lambda: L.matmul_rows(0, 1, a, b, 128, out),
+                lambda: L.matmul_rows(0, 1, a, b, 64, out[:, :5]), lambda: L.matmul_rows(0, 1, a.float(), b, 64, out),
+                lambda: L.matmul_rows(0, 1, a, b, 64, out.double()), lambda: L.matmul_rows(0, 1, a, b, 0, out),
+                lambda: L.matmul_rows(0, 1, a[:, 4:], b, 60, out), lambda: L.matmul_rows(0, 1, a, b.cpu(), 64, out)):
+        with pytest.raises(L.LegionError):
+            bad()
+    long = torch.zeros(1, 131088, dtype=torch.uint8, device="cuda")
+    with pytest.raises(L.LegionError, match="limit"):
+        L.matmul_rows(0, 1, long, long, 131072, torch.zeros(1, 1, device="cuda"))
+    assert bool((out == 3.0).all())
