@@ -384,6 +384,7 @@ _dtypes = {}
 
 
 def _code_of(dtype):
+    """(code of a float type or -1, bytes of an integer type or 0)"""
     if not _dtypes:
         import torch
         _dtypes.update({torch.float32: (F32, 0), torch.float16: (F16, 0), torch.bfloat16: (BF16, 0), torch.int32: (-1, 4),
@@ -391,27 +392,30 @@ def _code_of(dtype):
     return _dtypes.get(dtype, (-1, 0))
 
 
-def _operand(what, t, dev_id, dims, shape=None):
-    """Type code of a float tensor, after the checks that a pointer cannot make: where it lies, its shape, whole rows."""
-    if t.dim() != dims or (shape is not None and tuple(t.shape) != shape):
-        raise LegionError("%s: shape %s, expected %s" % (what, tuple(t.shape), shape if shape is not None else "%d dimensions" % dims))
+def _refused(what, t, dev_id, dims, shape):
+    if t.dim() != dims or (shape is not None and tuple(t.shape) != tuple(shape)):
+        return LegionError("%s: shape %s, expected %s" % (what, tuple(t.shape), tuple(shape) if shape is not None else "%d dimensions" % dims))
     if not t.is_cuda or t.get_device() != dev_id:
-        raise LegionError("%s is on %s, the call is for cuda:%d" % (what, t.device, dev_id))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise LegionError("%s: the elements of a row must lie one behind the other" % what)
-    return _code_of(t.dtype)
+        return LegionError("%s is on %s, the call is for cuda:%d" % (what, t.device, dev_id))
+    return LegionError("%s: the elements of a row must lie one behind the other" % what)
+
+
+def _operand(what, t, dev_id, dims, shape=None):
+    """Type code of a tensor, after the checks that a pointer cannot make: where it lies, its shape, whole rows."""
+    s = t.shape
+    if len(s) != dims or (shape is not None and s != shape) or t.get_device() != dev_id or not t.is_cuda or (s[-1] > 1 and t.stride(-1) != 1):
+        raise _refused(what, t, dev_id, dims, shape)
+    return _dtypes.get(t.dtype) or _code_of(t.dtype)
 
 
 def _rows(what, t, dev_id, shape=None):
+    """(type code, elements from row to row) of float rows; one row (or none) has no next one."""
     code = _operand(what, t, dev_id, 2, shape)[0]
     if code < 0:
         raise LegionError("%s: %s is not float32, float16 or bfloat16" % (what, t.dtype))
-    return code
-
-
-def _row_stride(t):
-    """Elements from row to row; one row (or none) has no next one."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    n, dim = t.shape
+    step = t.stride(0)
+    return code, step if n > 1 or step >= dim else dim
 
 
 def _id_width(what, ids, dev_id):
@@ -445,9 +449,12 @@ def _handle(stream):
 def embedding_lookup(dev_id, table, ids, out, scale=1.0, stream=None):
     """out[i] = scale * table[ids[i]] for a table [nodes, dim] of learned rows; an id outside the table gives a row of zeros.
     table and out: float32, float16 or bfloat16, each its own; ids: int32 or int64."""
-    td, od, width = _rows("table", table, dev_id), _rows("out", out, dev_id, (ids.shape[0], table.shape[1])), _id_width("ids", ids, dev_id)
-    _check(lib().legion_embedding_lookup(dev_id, table.data_ptr(), td, _row_stride(table), table.shape[0], ids.data_ptr(), width,
-                                         ids.shape[0], table.shape[1], scale, out.data_ptr(), od, _row_stride(out), _handle(stream)))
+    td, ts = _rows("table", table, dev_id)
+    width = _id_width("ids", ids, dev_id)
+    n, (nodes, dim) = ids.shape[0], table.shape
+    od, os_ = _rows("out", out, dev_id, (n, dim))
+    _check((_lib or lib()).legion_embedding_lookup(dev_id, table.data_ptr(), td, ts, nodes, ids.data_ptr(), width, n, dim, scale,
+                                                   out.data_ptr(), od, os_, _handle(stream)))
 
 
 def embedding_grad_workspace(n_ids, dim, n_nodes):
@@ -460,52 +467,60 @@ def embedding_grad_workspace(n_ids, dim, n_nodes):
 def embedding_grad(dev_id, ids, grad_out, grad_table, workspace, scale=1.0, accumulate=False, stream=None):
     """grad_table[v] = scale * sum of grad_out[i] over ids[i] == v, or added to what grad_table holds.  Ids outside the table
     are left out."""
-    gd, td, width = _rows("grad_out", grad_out, dev_id, (ids.shape[0], grad_table.shape[1])), _rows("grad_table", grad_table, dev_id), \
-        _id_width("ids", ids, dev_id)
+    width = _id_width("ids", ids, dev_id)
+    td, ts = _rows("grad_table", grad_table, dev_id)
+    n, (nodes, dim) = ids.shape[0], grad_table.shape
+    gd, gs = _rows("grad_out", grad_out, dev_id, (n, dim))
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check(lib().legion_embedding_grad(dev_id, ids.data_ptr(), width, ids.shape[0], grad_out.data_ptr(), gd, _row_stride(grad_out),
-                                       grad_table.shape[1], scale, grad_table.data_ptr(), td, _row_stride(grad_table),
-                                       grad_table.shape[0], 1 if accumulate else 0, ws, ws_bytes, _handle(stream)))
+    _check((_lib or lib()).legion_embedding_grad(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale,
+                                                 grad_table.data_ptr(), td, ts, nodes, 1 if accumulate else 0, ws, ws_bytes, _handle(stream)))
 
 
 def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, count, workspace, scale=1.0, stream=None):
     """The gradient's rows that occur: unique_ids[:count] rising, grad_rows[:count] their float32 gradients; count is one
     int32 on the device.  What lies behind count is left as it was."""
+    width = _id_width("ids", ids, dev_id)
+    gd, gs = _rows("grad_out", grad_out, dev_id)
     n, dim = grad_out.shape
-    gd, width = _rows("grad_out", grad_out, dev_id, (ids.shape[0], dim)), _id_width("ids", ids, dev_id)
-    if _rows("grad_rows", grad_rows, dev_id) != F32 or grad_rows.shape[0] < n or grad_rows.shape[1] != dim:
+    if ids.shape[0] != n:
+        raise LegionError("grad_out: %d rows for %d ids" % (n, ids.shape[0]))
+    rd, rs = _rows("grad_rows", grad_rows, dev_id)
+    if rd != F32 or grad_rows.shape[0] < n or grad_rows.shape[1] != dim:
         raise LegionError("grad_rows must be float32, with a row for every id")
     if _id_width("unique_ids", unique_ids, dev_id) != width or unique_ids.shape[0] < n:
         raise LegionError("unique_ids must be as wide as ids, with an entry for every id")
     if _operand("count", count, dev_id, 1, (1,)) != (-1, 4):
         raise LegionError("count must be one int32")
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check(lib().legion_embedding_grad_rows(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, _row_stride(grad_out), dim, scale,
-                                            n_nodes, unique_ids.data_ptr(), grad_rows.data_ptr(), _row_stride(grad_rows),
-                                            count.data_ptr(), ws, ws_bytes, _handle(stream)))
+    _check((_lib or lib()).legion_embedding_grad_rows(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale, n_nodes,
+                                                      unique_ids.data_ptr(), grad_rows.data_ptr(), rs, count.data_ptr(), ws, ws_bytes,
+                                                      _handle(stream)))
 
 
 def rms_norm(dev_id, x, weight, out, eps=1e-6, residual=None, residual_out=None, codec=CODEC_RAW, stream=None):
     """h = x + residual; out = h * weight / sqrt(mean(h^2) + eps); residual_out = h.  codec CODEC_INT8 or CODEC_E4M3: out is uint8
     and receives the compressed rows that quantize_table would make of the float32 result."""
-    dt = _rows("x", x, dev_id)
-    n, dim = x.shape
+    dt, xs = _rows("x", x, dev_id)
+    shape = n, dim = x.shape
     wd = _operand("weight", weight, dev_id, 1, (dim,))[0]
-    for what, t in (("residual", residual), ("residual_out", residual_out)):
-        if t is not None and _rows(what, t, dev_id, (n, dim)) != dt:
-            raise LegionError("%s must be of x's type" % what)
+    rp = rs = tp = ts = 0
+    rd = td = dt
+    if residual is not None:
+        rd, rs = _rows("residual", residual, dev_id, shape)
+        rp = residual.data_ptr()
+    if residual_out is not None:
+        td, ts = _rows("residual_out", residual_out, dev_id, shape)
+        tp = residual_out.data_ptr()
     if codec == CODEC_RAW:
-        if _rows("out", out, dev_id, (n, dim)) != dt:
-            raise LegionError("out must be of x's type")
-        stride = _row_stride(out)
+        od, os_ = _rows("out", out, dev_id, shape)
     else:
-        stride = _code_rows("out", out, dev_id, dim)
+        od, os_ = dt, _code_rows("out", out, dev_id, dim)
         if out.shape[0] != n:
             raise LegionError("out: %d rows, expected %d" % (out.shape[0], n))
-    _check(lib().legion_rms_norm(dev_id, x.data_ptr(), dt, _row_stride(x), None if residual is None else residual.data_ptr(),
-                                 0 if residual is None else _row_stride(residual), weight.data_ptr(), wd, eps, n, dim, codec,
-                                 out.data_ptr(), stride, None if residual_out is None else residual_out.data_ptr(),
-                                 0 if residual_out is None else _row_stride(residual_out), _handle(stream)))
+    if rd != dt or td != dt or od != dt:
+        raise LegionError("residual, residual_out and out must be of x's type")
+    _check((_lib or lib()).legion_rms_norm(dev_id, x.data_ptr(), dt, xs, rp or None, rs, weight.data_ptr(), wd, eps, n, dim, codec,
+                                           out.data_ptr(), os_, tp or None, ts, _handle(stream)))
 
 
 def rms_norm_grad_workspace(n_rows, dim):
@@ -518,17 +533,20 @@ def rms_norm_grad_workspace(n_rows, dim):
 def rms_norm_grad(dev_id, grad_out, x, weight, grad_x, grad_weight, workspace, eps=1e-6, grad_residual=None, stream=None):
     """Gradients of rms_norm at the rows x that were normed (its residual_out, if it had a residual).  grad_residual: what reached
     residual_out by other ways, added to grad_x."""
-    dt = _rows("x", x, dev_id)
-    n, dim = x.shape
-    for what, t in (("grad_out", grad_out), ("grad_x", grad_x), ("grad_residual", grad_residual)):
-        if (t is not None or what != "grad_residual") and _rows(what, t, dev_id, (n, dim)) != dt:
-            raise LegionError("%s must be of x's type" % what)
-    wd, gd = _operand("weight", weight, dev_id, 1, (dim,))[0], _operand("grad_weight", grad_weight, dev_id, 1, (dim,))[0]
+    dt, xs = _rows("x", x, dev_id)
+    shape = n, dim = x.shape
+    gd, gs = _rows("grad_out", grad_out, dev_id, shape)
+    od, os_ = _rows("grad_x", grad_x, dev_id, shape)
+    rd, rs, rp = dt, 0, None
+    if grad_residual is not None:
+        rd, rs = _rows("grad_residual", grad_residual, dev_id, shape)
+        rp = grad_residual.data_ptr() or None
+    if gd != dt or od != dt or rd != dt:
+        raise LegionError("grad_out, grad_x and grad_residual must be of x's type")
+    wd, wg = _operand("weight", weight, dev_id, 1, (dim,))[0], _operand("grad_weight", grad_weight, dev_id, 1, (dim,))[0]
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check(lib().legion_rms_norm_grad(dev_id, grad_out.data_ptr(), _row_stride(grad_out), x.data_ptr(), _row_stride(x), dt,
-                                      None if grad_residual is None else grad_residual.data_ptr(),
-                                      0 if grad_residual is None else _row_stride(grad_residual), weight.data_ptr(), wd, eps, n, dim,
-                                      grad_x.data_ptr(), _row_stride(grad_x), grad_weight.data_ptr(), gd, ws, ws_bytes, _handle(stream)))
+    _check((_lib or lib()).legion_rms_norm_grad(dev_id, grad_out.data_ptr(), gs, x.data_ptr(), xs, dt, rp, rs, weight.data_ptr(), wd, eps, n,
+                                                dim, grad_x.data_ptr(), os_, grad_weight.data_ptr(), wg, ws, ws_bytes, _handle(stream)))
 
 
 def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None):
@@ -536,9 +554,9 @@ def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None)
     feature_len codes (rms_norm, quantize_table, a cache's partition); out: float32, float16 or bfloat16."""
     rs, ws = _code_rows("rows", rows, dev_id, feature_len), _code_rows("weight_rows", weight_rows, dev_id, feature_len)
     m, n = rows.shape[0], weight_rows.shape[0]
-    od = _rows("out", out, dev_id, (m, n))
-    _check(lib().legion_matmul_rows(dev_id, codec, rows.data_ptr(), m, rs, weight_rows.data_ptr(), n, ws, feature_len, out.data_ptr(), od,
-                                    _row_stride(out), _handle(stream)))
+    od, os_ = _rows("out", out, dev_id, (m, n))
+    _check((_lib or lib()).legion_matmul_rows(dev_id, codec, rows.data_ptr(), m, rs, weight_rows.data_ptr(), n, ws, feature_len,
+                                              out.data_ptr(), od, os_, _handle(stream)))
 
 
 def operator_error(dev_id, stream=None, reset=True):

@@ -59,6 +59,29 @@ struct NormParams {
     float eps;
 };
 
+// VE weights in fp32, by vectors where the address allows it; zeros behind the row's end.
+template <typename T, int VE>
+__device__ __forceinline__ void load_weight(const void *p, int dtype, int col, int dim, float *w)
+{
+    if (col >= dim) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = 0.0f;
+    } else if (dtype == LEGION_F32 && (uintptr_t)p % 16 == 0) {   // col is a multiple of VE
+        Vec<float, VE> v;
+        v.load(static_cast<const float *>(p) + col);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = v.get(i);
+    } else if (dtype != LEGION_F32 && (uintptr_t)p % 16 == 0) {
+        Vec<T, VE> v;
+        v.load(static_cast<const T *>(p) + col);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = v.get(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = load_any(p, dtype, col + i);
+    }
+}
+
 template <int VE>
 __device__ __forceinline__ void store_codes(uint8_t *p, const uint32_t *c)
 {
@@ -76,51 +99,56 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
     const int width = GROUP == 0 ? blockDim.x : GROUP;
     const int t = GROUP == 0 ? threadIdx.x : threadIdx.x & (GROUP - 1);
     const int per_cta = GROUP == 0 ? 1 : 128 / (GROUP == 0 ? 1 : GROUP);
+    const int mate = GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP);
+    Vec<T, VE> a[U], r[U];
+    auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            a[u].zero();
+            r[u].zero();
+            if (row < p.n && col < p.dim) {
+                a[u].load(static_cast<const T *>(p.x) + row * p.x_stride + col);
+                if (p.residual != nullptr) r[u].load(static_cast<const T *>(p.residual) + row * p.residual_stride + col);
+            }
+        }
+    };
+    constexpr bool kAhead = U * VE <= 16;   // wider threads have no registers for it
+    const int64_t step = (int64_t)gridDim.x * per_cta;
+    if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
     float w[U][VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int col = (t + u * width) * VE;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) w[u][i] = col < p.dim ? load_any(p.weight, p.weight_dtype, col + i) : 0.0f;
-    }
+    for (int u = 0; u < U; ++u) load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, w[u]);
     const float top = CODEC == LEGION_CODEC_INT8 ? 127.0f : 448.0f;
     // the rows of a CTA's groups end together, so that every lane takes part in the reductions
-    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += (int64_t)gridDim.x * per_cta) {
-        const int64_t row = row0 + (GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP));
+    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += step) {
+        const int64_t row = row0 + mate;
         const bool in = row < p.n;
+        if (!kAhead) fetch(row);
         float h[U][VE];
         float sum = 0.0f, most = 0.0f;
-        {
-            Vec<T, VE> a[U], r[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int col = (t + u * width) * VE;
-                a[u].zero();
-                if (in && col < p.dim) a[u].load(static_cast<const T *>(p.x) + row * p.x_stride + col);
-                if (p.residual != nullptr) {
-                    r[u].zero();
-                    if (in && col < p.dim) r[u].load(static_cast<const T *>(p.residual) + row * p.residual_stride + col);
-                }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                h[u][i] = a[u].get(i);
+                if (p.residual != nullptr) h[u][i] += r[u].get(i);
+            }
+        if (kAhead && row0 + step < p.n) fetch(row + step);  // the next row is on its way while this one is worked on
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) sum = fmaf(h[u][i], h[u][i], sum);
+            if (p.residual_out != nullptr && in && col < p.dim) {
+                Vec<T, VE> o;
+                o.set(h[u]);
+                o.store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride + col);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int col = (t + u * width) * VE;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    h[u][i] = a[u].get(i);
-                    if (p.residual != nullptr) h[u][i] += r[u].get(i);
-                    sum = fmaf(h[u][i], h[u][i], sum);
-                }
-                if (p.residual_out != nullptr && in && col < p.dim) {
-                    Vec<T, VE> o;
-                    o.set(h[u]);
-                    o.store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride + col);
-                }
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    h[u][i] *= w[u][i];
-                    if (CODEC != LEGION_CODEC_RAW && col < p.dim) most = max_nan(most, fabsf(h[u][i]));
-                }
+            for (int i = 0; i < VE; ++i) {
+                h[u][i] *= w[u][i];
+                if (CODEC != LEGION_CODEC_RAW && col < p.dim) most = max_nan(most, fabsf(h[u][i]));
             }
         }
         reduce.two(sum, most, true);
@@ -193,34 +221,45 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
     const int width = GROUP == 0 ? blockDim.x : GROUP;
     const int t = GROUP == 0 ? threadIdx.x : threadIdx.x & (GROUP - 1);
     const int per_cta = GROUP == 0 ? 1 : 128 / (GROUP == 0 ? 1 : GROUP);
-    float w[U][VE], dw[U][VE];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int col = (t + u * width) * VE;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            w[u][i] = col < p.dim ? load_any(p.weight, p.weight_dtype, col + i) : 0.0f;
-            dw[u][i] = 0.0f;
-        }
-    }
-    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += (int64_t)gridDim.x * per_cta) {
-        const int64_t row = row0 + (GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP));
-        const bool in = row < p.n;
-        Vec<T, VE> h[U], dy[U], r[U];
-        float square = 0.0f, dot = 0.0f;
+    const int mate = GROUP == 0 ? 0 : threadIdx.x / (GROUP == 0 ? 1 : GROUP);
+    Vec<T, VE> next_h[U], next_dy[U], next_r[U];
+    auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int col = (t + u * width) * VE;
-            h[u].zero();
-            dy[u].zero();
-            if (p.grad_residual != nullptr) r[u].zero();
-            if (in && col < p.dim) {
-                h[u].load_stream(static_cast<const T *>(p.x) + row * p.x_stride + col);
-                dy[u].load_stream(static_cast<const T *>(p.grad_out) + row * p.grad_stride + col);
-                if (p.grad_residual != nullptr)
-                    r[u].load(static_cast<const T *>(p.grad_residual) + row * p.grad_residual_stride + col);
+            next_h[u].zero();
+            next_dy[u].zero();
+            next_r[u].zero();
+            if (row < p.n && col < p.dim) {
+                next_h[u].load(static_cast<const T *>(p.x) + row * p.x_stride + col);
+                next_dy[u].load(static_cast<const T *>(p.grad_out) + row * p.grad_stride + col);
+                if (p.grad_residual != nullptr) next_r[u].load(static_cast<const T *>(p.grad_residual) + row * p.grad_residual_stride + col);
             }
         }
+    };
+    constexpr bool kAhead = U * VE <= 16;   // wider threads have no registers for it
+    const int64_t step = (int64_t)gridDim.x * per_cta;
+    if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
+    float w[U][VE], dw[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, w[u]);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) dw[u][i] = 0.0f;
+    }
+    for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += step) {
+        const int64_t row = row0 + mate;
+        const bool in = row < p.n;
+        if (!kAhead) fetch(row);
+        Vec<T, VE> h[U], dy[U], r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            h[u] = next_h[u];
+            dy[u] = next_dy[u];
+            r[u] = next_r[u];
+        }
+        if (kAhead && row0 + step < p.n) fetch(row + step);  // the next row is on its way while this one is worked on
+        float square = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -280,7 +319,7 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float *__r
     const int col = blockIdx.x * 32 + x;
     float sum = 0.0f;
     if (col < dim)
-#pragma unroll 4
+#pragma unroll 8
         for (int g = y; g < parts; g += 32) sum += part[(int64_t)g * dim + col];
     s[y][x] = sum;
     __syncthreads();
@@ -306,8 +345,18 @@ static RowShape row_shape(int vecs, int64_t n)
     int u = 1;  // few rows: as many threads as there are vectors; many: CTAs of about 256 threads, so that several are on an SM
     if (n >= 2 * kSms)
         while (u < 4 && (vecs + u - 1) / u > 256) u *= 2;
-    while ((vecs + u - 1) / u > 1024) u *= 2;
+    while ((vecs + u - 1) / u > 512) u *= 2;
     return { 0, u, ((vecs + u - 1) / u + 31) / 32 * 32, 1 };
+}
+
+// CTAs of a kernel that loops over rows: as many as are on the chip at one time (at most `per_sm` a SM), so that none starts late.
+static unsigned resident(int64_t need, const void *kernel, int threads, int per_sm)
+{
+    if (need <= kSms) return (unsigned)need;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, 0) != cudaSuccess || fit < 1) fit = 1;
+    if (fit > per_sm) fit = per_sm;
+    return (unsigned)(need < (int64_t)fit * kSms ? need : (int64_t)fit * kSms);
 }
 
 template <typename T, int VE, int CODEC>
@@ -315,18 +364,19 @@ static int launch_norm(cudaStream_t s, const NormParams &p)
 {
     const RowShape r = row_shape(p.dim / VE, p.n);
     const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
-    const int64_t most = (int64_t)kSms * (2048 / r.threads);
-    const unsigned grid = (unsigned)(need < most ? need : most);
-#define LG_NORM(U, GROUP, MAXT) norm_kernel<T, VE, U, GROUP, CODEC, MAXT><<<grid, r.threads, 0, s>>>(p)
-// registers are what a CTA of 1024 threads lacks: rows that smaller CTAs hold get kernels with more of them
-#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, (U * VE > 16 ? 512 : 1024)); } while (0)
+#define LG_NORM(U, GROUP, MAXT)                                                                                                     \
+    norm_kernel<T, VE, U, GROUP, CODEC, MAXT><<<resident(need, (const void *)norm_kernel<T, VE, U, GROUP, CODEC, MAXT>, r.threads, 16), \
+                                                r.threads, 0, s>>>(p)
+// a CTA of at most 256 threads may have twice the registers of a thread of one of 512
+#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, 512); } while (0)
     if (r.group == 8) LG_NORM(1, 8, 128);
     else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
     else if (r.u == 1) LG_NORM_CTA(1);
     else if (r.u == 2) LG_NORM_CTA(2);
     else if (r.u == 4) LG_NORM_CTA(4);
-    else if (r.u == 8) { if constexpr (VE <= 2) LG_NORM(8, 0, 1024); }
-    else { if constexpr (VE == 1) LG_NORM(16, 0, 1024); }
+    else if (r.u == 8) { if constexpr (VE <= 4) LG_NORM(8, 0, 512); }
+    else if (r.u == 16) { if constexpr (VE <= 2) LG_NORM(16, 0, 512); }
+    else { if constexpr (VE == 1) LG_NORM(32, 0, 512); }
 #undef LG_NORM_CTA
 #undef LG_NORM
     LG_LAUNCH_CHECK();
@@ -358,18 +408,19 @@ static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
 {
     const RowShape r = row_shape(p.dim / VE, p.n);
     const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
-    const unsigned grid = (unsigned)(need < kGradCtas ? need : kGradCtas);
-    *parts = (int)grid;
-#define LG_NORM(U, GROUP, MAXT) norm_grad_kernel<T, VE, U, GROUP, MAXT><<<grid, r.threads, 0, s>>>(p)
-// registers are what a CTA of 1024 threads lacks: rows that smaller CTAs hold get kernels with more of them
-#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, (U * VE > 16 ? 512 : 1024)); } while (0)
+#define LG_NORM(U, GROUP, MAXT)                                                                                                    \
+    norm_grad_kernel<T, VE, U, GROUP, MAXT><<<*parts = resident(need, (const void *)norm_grad_kernel<T, VE, U, GROUP, MAXT>, r.threads, \
+                                                                kGradCtas / kSms), r.threads, 0, s>>>(p)
+// a CTA of at most 256 threads may have twice the registers of a thread of one of 512
+#define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, 512); } while (0)
     if (r.group == 8) LG_NORM(1, 8, 128);
     else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
     else if (r.u == 1) LG_NORM_CTA(1);
     else if (r.u == 2) LG_NORM_CTA(2);
     else if (r.u == 4) LG_NORM_CTA(4);
-    else if (r.u == 8) { if constexpr (VE <= 2) LG_NORM(8, 0, 1024); }
-    else { if constexpr (VE == 1) LG_NORM(16, 0, 1024); }
+    else if (r.u == 8) { if constexpr (VE <= 4) LG_NORM(8, 0, 512); }
+    else if (r.u == 16) { if constexpr (VE <= 2) LG_NORM(16, 0, 512); }
+    else { if constexpr (VE == 1) LG_NORM(32, 0, 512); }
 #undef LG_NORM_CTA
 #undef LG_NORM
     LG_LAUNCH_CHECK();
