@@ -410,12 +410,14 @@ def _operand(what, t, dev_id, dims, shape=None):
 
 def _rows(what, t, dev_id, shape=None):
     """(type code, elements from row to row) of float rows; one row (or none) has no next one."""
-    code = _operand(what, t, dev_id, 2, shape)[0]
+    s, step = t.shape, t.stride()
+    if len(s) != 2 or (shape is not None and s != shape) or t.get_device() != dev_id or not t.is_cuda or (s[1] > 1 and step[1] != 1):
+        raise _refused(what, t, dev_id, 2, shape)
+    code = (_dtypes.get(t.dtype) or _code_of(t.dtype))[0]
     if code < 0:
         raise LegionError("%s: %s is not float32, float16 or bfloat16" % (what, t.dtype))
-    n, dim = t.shape
-    step = t.stride(0)
-    return code, step if n > 1 or step >= dim else dim
+    n, dim = s
+    return code, step[0] if n > 1 or step[0] >= dim else dim
 
 
 def _id_width(what, ids, dev_id):

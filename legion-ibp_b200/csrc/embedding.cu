@@ -102,65 +102,242 @@ static void launch_lookup_to(int out_dtype, int ve, cudaStream_t s, const Ids &i
 
 // ---- sort ----------------------------------------------------------------------------------------------------------
 
-constexpr int kRankMax = 8192;   // lists up to here are sorted by counting, in one launch
 constexpr int kDigits = 256;
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterItems = 11;                            // entries that a thread has at most
+constexpr int kClusterPart = kClusterItems * kClusterThreads; // entries that a CTA has at most
+constexpr int kHistPitch = kDigits + 1;                      // the 32 counts of a digit lie in 32 banks
 
-// The place of entry i in the sorted list is the number of entries that come before it: those with a smaller key, and
-// those with the same key and a smaller position.  A CTA has 64 entries and a quarter of the list per 64 threads.
-// n^2 comparisons, but one launch and no dependence: 8192 entries are 2^26 comparisons over 148 SMs.
-__global__ void __launch_bounds__(256) rank_sort_kernel(Ids ids, int n, uint32_t *keys, int32_t *pos)
+// The rows of the gradient that no id names are zeros: the CTAs of the sorting launch that have nothing to sort write them (all
+// rows; those that are named are written again by the sums).
+struct ZeroFill {
+    uint8_t *p;            // nullptr: nothing to fill
+    int64_t rows, width, pitch;  // bytes of a row, bytes from row to row
+};
+
+// `threads` threads write `bytes` zero bytes from p on (both multiples of two).
+__device__ __forceinline__ void zero_run(uint8_t *p, int64_t bytes, int64_t at, int64_t threads)
 {
-    __shared__ uint32_t tile[1024];
-    __shared__ int part[256];
-    const int t = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const int i = blockIdx.x * 64 + t;
-    const uint32_t mine = i < n ? ids.key(i) : 0;
-    int before = 0;
-    for (int j0 = 0; j0 < n; j0 += 1024) {
-        __syncthreads();
-        for (int j = threadIdx.x; j < 1024; j += 256) tile[j] = j0 + j < n ? ids.key(j0 + j) : 0xFFFFFFFFu;
-        __syncthreads();
-        const int lo = j0 + q * 256;
-        const uint4 *four = reinterpret_cast<const uint4 *>(tile + q * 256);
-        if (lo + 256 <= (int)blockIdx.x * 64) {        // all of them stand before entry i
-#pragma unroll 8
-            for (int j = 0; j < 64; ++j) {
-                const uint4 k = four[j];
-                before += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
-            }
-        } else if (lo >= (int)blockIdx.x * 64 + 64) {  // behind it
-#pragma unroll 8
-            for (int j = 0; j < 64; ++j) {
-                const uint4 k = four[j];
-                before += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
-            }
-        } else {
-            for (int j = 0; j < 256; ++j) {
-                const uint32_t k = tile[q * 256 + j];
-                before += (k < mine) || (k == mine && lo + j < i);
-            }
-        }
-    }
-    part[threadIdx.x] = before;
-    __syncthreads();
-    if (q == 0 && i < n) {
-        const int at = part[t] + part[t + 64] + part[t + 128] + part[t + 192];
-        keys[at] = mine;
-        pos[at] = i;
+    int64_t head = (16 - ((uintptr_t)p & 15)) & 15;
+    if (head > bytes) head = bytes;
+    const int64_t vecs = (bytes - head) / 16, tail = bytes - head - vecs * 16;
+    if (at * 2 < head) reinterpret_cast<uint16_t *>(p)[at] = 0;
+    uint4 *v = reinterpret_cast<uint4 *>(p + head);
+    for (int64_t i = at; i < vecs; i += threads) __stcs(v + i, make_uint4(0, 0, 0, 0));
+    if (at * 2 < tail) reinterpret_cast<uint16_t *>(p + head + vecs * 16)[at] = 0;
+}
+__device__ __forceinline__ void zero_fill(const ZeroFill &z, int64_t at, int64_t threads)
+{
+    if (z.p == nullptr) return;
+    if (z.pitch == z.width) {
+        zero_run(z.p, z.rows * z.width, at, threads);
+    } else {
+        for (int64_t r = at >> 5; r < z.rows; r += threads >> 5) zero_run(z.p + r * z.pitch, z.width, at & 31, 32);
     }
 }
 
-// Longer lists: least significant digit first, 8 bits a pass, every CTA one contiguous part of the list.
+// Lanes of the warp whose digit is this lane's, by one vote a bit (a match instruction takes a step per different digit).
+__device__ __forceinline__ unsigned same_digit(int digit, bool in)
+{
+    unsigned same = __ballot_sync(kFull, in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const unsigned ones = __ballot_sync(kFull, (digit >> b) & 1);
+        same &= (digit >> b) & 1 ? ones : ~ones;
+    }
+    return same;
+}
+
+struct ClusterSort {
+    Ids ids;
+    int32_t n, part;      // entries; entries per CTA, a multiple of kClusterThreads
+    FastDiv per_part;
+    int32_t bits;
+    uint2 *pairs;         // sorted: (key, position)
+    int32_t *heads;       // rows that occur: first entries before every stretch (GradOut), or nullptr
+    int32_t *count;
+    int32_t stretch;      // a multiple of 32
+    ZeroFill fill;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of the same shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(const void *p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ int32_t load_cta(uint32_t a)
+{
+    int32_t v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_cta(uint32_t a, uint2 v)
+{
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
+}
+
+__host__ __device__ constexpr int64_t cluster_sort_smem(int64_t part) { return part * 16 + 4 * (32 * kHistPitch + 2 * kDigits + 80); }
+
+// Stable sort by least significant digit, eight bits a pass, inside the shared memory of one cluster: no launch and no global memory
+// between the passes.  A warp has 32 * items entries one behind the other and ranks them in list order; counts of
+// the CTAs' digits are read out of each other's shared memory, entries are written straight to the CTA that has their place.
+// What bounds it is latency (two cluster barriers a pass), so the entries are spread over up to 16 CTAs even when one could hold them.
+// Clusters behind the first one write the zero rows of the gradient meanwhile.
+__global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(ClusterSort p)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t size = cluster_size();
+    if (blockIdx.x >= size) {
+        zero_fill(p.fill, (int64_t)(blockIdx.x - size) * kClusterThreads + threadIdx.x, (int64_t)(gridDim.x - size) * kClusterThreads);
+        return;
+    }
+    const uint32_t me = cluster_rank();
+    uint2 *buf[2] = { reinterpret_cast<uint2 *>(smem), reinterpret_cast<uint2 *>(smem) + p.part };
+    int32_t *hist = reinterpret_cast<int32_t *>(buf[1] + p.part);  // [warp][digit]
+    int32_t *total = hist + 32 * kHistPitch;                       // entries of each digit in this CTA; read by the others
+    int32_t *base = total + kDigits;                               // where the CTA's first entry of a digit goes
+    int32_t *scan = base + kDigits;                                // 32 words and a word that the others read
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int first = (int)me * p.part, mine = max(0, min(p.part, p.n - first));
+    const int items = p.part / kClusterThreads;
+    const int at0 = warp * 32 * items + lane;                      // the lane's first entry; the next ones are 32 apart
+    for (int i = threadIdx.x; i < mine; i += kClusterThreads) buf[0][i] = make_uint2(p.ids.key(first + i), (uint32_t)(first + i));
+    int cur = 0;
+    for (int shift = 0; shift < p.bits; shift += 8, cur ^= 1) {
+        for (int i = threadIdx.x; i < 32 * kHistPitch; i += kClusterThreads) hist[i] = 0;
+        __syncthreads();
+        uint16_t rank[kClusterItems];  // among the warp's entries of the same digit
+#pragma unroll
+        for (int j = 0; j < kClusterItems; ++j) {
+            if (j < items) {
+                const int i = at0 + j * 32;
+                const bool in = i < mine;
+                const int digit = in ? (int)((buf[cur][i].x >> shift) & (kDigits - 1)) : 0;
+                const unsigned same = same_digit(digit, in);
+                const int before = hist[warp * kHistPitch + digit];
+                __syncwarp();
+                const int among = __popc(same & ((1u << lane) - 1u));
+                if (in && among == 0) hist[warp * kHistPitch + digit] = before + __popc(same);
+                __syncwarp();
+                rank[j] = (uint16_t)(before + among);
+            }
+        }
+        __syncthreads();
+        {   // counts of the warps -> entries of the digit in the warps before; four threads a digit, eight warps each
+            const int d = threadIdx.x >> 2, q = threadIdx.x & 3;
+            int v[8], sum = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = hist[(q * 8 + k) * kHistPitch + d];
+                sum += v[k];
+            }
+            int incl = sum;
+            int o = __shfl_up_sync(kFull, incl, 1, 4);
+            if (q >= 1) incl += o;
+            o = __shfl_up_sync(kFull, incl, 2, 4);
+            if (q >= 2) incl += o;
+            int run = incl - sum;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                hist[(q * 8 + k) * kHistPitch + d] = run;
+                run += v[k];
+            }
+            if (q == 3) total[d] = incl;
+        }
+        cluster_sync();
+        {   // entries of smaller digits anywhere, and of the same digit in the CTAs before; four threads a digit
+            const int d = threadIdx.x >> 2, q = threadIdx.x & 3;
+            int all = 0, before = 0;
+            for (uint32_t c = q; c < size; c += 4) {
+                const int v = load_cta(in_cta(total + d, c));
+                all += v;
+                before += c < me ? v : 0;
+            }
+            all += __shfl_xor_sync(kFull, all, 1);
+            all += __shfl_xor_sync(kFull, all, 2);
+            before += __shfl_xor_sync(kFull, before, 1);
+            before += __shfl_xor_sync(kFull, before, 2);
+            int incl = q == 0 ? all : 0;   // sum over the digits up to d
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const int o = __shfl_up_sync(kFull, incl, s);
+                if (lane >= s) incl += o;
+            }
+            if (lane == 31) scan[warp] = incl;
+            __syncthreads();
+            const int warps_before = __reduce_add_sync(kFull, lane < warp ? scan[lane] : 0);
+            if (q == 0) base[d] = warps_before + incl - all + before;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kClusterItems; ++j) {
+            const int i = at0 + j * 32;
+            if (j < items && i < mine) {
+                const uint2 e = buf[cur][i];
+                const int digit = (int)((e.x >> shift) & (kDigits - 1));
+                const uint32_t to = (uint32_t)(base[digit] + hist[warp * kHistPitch + digit] + rank[j]);
+                const uint32_t cta = p.per_part.div(to);
+                store_cta(in_cta(buf[cur ^ 1] + (to - cta * (uint32_t)p.part), cta), e);
+            }
+        }
+        cluster_sync();
+    }
+    const uint2 *sorted = buf[cur];
+    for (int i = threadIdx.x; i < mine; i += kClusterThreads) p.pairs[first + i] = sorted[i];
+    if (p.heads != nullptr) {
+        // first entries of 32 entries each: at most kClusterPart / 32 counts, one thread each
+        const int pieces = p.part / 32;
+        int32_t *count = hist;
+        for (int k = warp; k < pieces; k += 32) {
+            const int i = k * 32 + lane;
+            bool head = i < mine && sorted[i].x < (uint32_t)p.ids.n_nodes;
+            if (head && first + i > 0)
+                head = sorted[i].x != (i > 0 ? sorted[i - 1].x : (uint32_t)load_cta(in_cta(&sorted[p.part - 1].x, me - 1)));
+            const unsigned all = __ballot_sync(kFull, head);
+            if (lane == 0) count[k] = __popc(all);
+        }
+        __syncthreads();
+        const int c = threadIdx.x < pieces ? count[threadIdx.x] : 0;
+        int incl = c;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int o = __shfl_up_sync(kFull, incl, s);
+            if (lane >= s) incl += o;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        const int of_cta = __reduce_add_sync(kFull, scan[lane]);
+        const int excl = __reduce_add_sync(kFull, lane < warp ? scan[lane] : 0) + incl - c;
+        if (threadIdx.x == 0) scan[32] = of_cta;
+        cluster_sync();
+        const int before = __reduce_add_sync(kFull, (uint32_t)lane < me ? load_cta(in_cta(scan + 32, lane)) : 0);
+        const int i = threadIdx.x * 32;
+        if (threadIdx.x < pieces && i < mine && (first + i) % p.stretch == 0) p.heads[(first + i) / p.stretch] = before + excl;
+        if (threadIdx.x == 0 && me == size - 1) {
+            p.heads[(p.n + p.stretch - 1) / p.stretch] = before + of_cta;
+            p.count[0] = before + of_cta;
+        }
+    }
+    cluster_sync();  // no CTA's memory goes while another one may read it
+}
+
+// Lists that no cluster holds: the same passes over global memory, every CTA one contiguous part of the list.
 struct SortPass {
     Ids ids;                  // first pass: the ids themselves
-    const uint32_t *keys_in;  // later ones: the pairs
-    const int32_t *pos_in;
-    uint32_t *keys_out;
-    int32_t *pos_out;
+    const uint2 *in;          // later ones: the pairs
+    uint2 *out;
     int32_t *counts;          // [CTA][digit]
     int64_t n, part;          // entries, entries per CTA
     int32_t shift;
-    __device__ __forceinline__ uint32_t key(int64_t i) const { return keys_in != nullptr ? keys_in[i] : ids.key(i); }
+    __device__ __forceinline__ uint2 pair(int64_t i) const { return in != nullptr ? in[i] : make_uint2(ids.key(i), (uint32_t)i); }
 };
 
 __global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p)
@@ -169,7 +346,7 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p)
     if (threadIdx.x < kDigits) hist[threadIdx.x] = 0;
     __syncthreads();
     const int64_t lo = blockIdx.x * p.part, hi = min(p.n, lo + p.part);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&hist[(p.key(i) >> p.shift) & (kDigits - 1)], 1);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&hist[(p.pair(i).x >> p.shift) & (kDigits - 1)], 1);
     __syncthreads();
     if (threadIdx.x < kDigits) p.counts[blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
 }
@@ -216,10 +393,9 @@ __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
         __syncthreads();
         const int64_t i = i0 + threadIdx.x;
         const bool in = i < hi;
-        const uint32_t key = in ? p.key(i) : 0u;
-        const int32_t at = in ? (p.pos_in != nullptr ? p.pos_in[i] : (int32_t)i) : 0;
-        const int digit = in ? (int)((key >> p.shift) & (kDigits - 1)) : kDigits;  // no entry: a digit of its own
-        const unsigned same = __match_any_sync(kFull, digit);
+        const uint2 e = in ? p.pair(i) : make_uint2(0, 0);
+        const int digit = in ? (int)((e.x >> p.shift) & (kDigits - 1)) : 0;
+        const unsigned same = same_digit(digit, in);
         const int rank = __popc(same & ((1u << lane) - 1u));
         if (in && rank == 0) whist[warp][digit] = __popc(same);
         __syncthreads();
@@ -234,23 +410,19 @@ __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
             base[d] = run;
         }
         __syncthreads();
-        if (in) {
-            const int to = whist[warp][digit] + rank;
-            p.keys_out[to] = key;
-            p.pos_out[to] = at;
-        }
+        if (in) p.out[whist[warp][digit] + rank] = e;
     }
 }
 
 // ---- sums over the sorted list -------------------------------------------------------------------------------------
 
 struct Sorted {
-    const uint32_t *keys;
-    const int32_t *pos;
+    const uint2 *pairs;   // (key, position)
     int64_t n;
     uint32_t n_nodes;     // the key of what is left out; such entries are the last ones
     int32_t stretch;      // entries that a group of threads sums
     int64_t stretches;
+    __device__ __forceinline__ uint32_t key(int64_t i) const { return pairs[i].x; }
 };
 
 // heads[c] = entries of stretch c that are the first of their id
@@ -261,8 +433,8 @@ __global__ void __launch_bounds__(256) head_count_kernel(Sorted l, int32_t *head
     if (c >= l.stretches) return;
     int count = 0;
     for (int64_t i = c * l.stretch + lane; i < min(l.n, (c + 1) * l.stretch); i += 32) {
-        const uint32_t k = l.keys[i];
-        count += k < l.n_nodes && (i == 0 || l.keys[i - 1] != k);
+        const uint32_t k = l.key(i);
+        count += k < l.n_nodes && (i == 0 || l.key(i - 1) != k);
     }
     count = __reduce_add_sync(kFull, count);
     if (lane == 0) heads[c] = count;
@@ -336,34 +508,62 @@ struct GradOut {
     }
 };
 
+constexpr int kSumThreads = 128;
+
+template <int VE>
+__device__ __forceinline__ void store_part(float *p, const float *x)
+{
+    Vec<float, VE> v;
+    v.set(x);
+    v.store(p);
+}
+template <int VE>
+__device__ __forceinline__ void load_part(const float *p, float *x)
+{
+    Vec<float, VE> v;
+    v.load(p);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) x[i] = v.get(i);
+}
+
 // 2^log_group threads have a stretch, one vector of VE columns each.  What bounds it is HBM: the rows of the gradient are read
-// once, `kAhead` of them in flight per thread, whatever ids they belong to; only the additions go one after the other.
+// once, `kAhead` of them on their way while the `kAhead` before them are added, whatever ids they belong to; only the additions
+// go one after the other.
 template <typename T, int VE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kSumThreads, 5)
 grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradOut o, int log_group)
 {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
     const int group = threadIdx.x >> log_group;
-    const int col = ((int)blockIdx.y * 256 + (threadIdx.x & ((1 << log_group) - 1))) * VE;
-    const int64_t c = ((int64_t)blockIdx.x << (8 - log_group)) + group;
+    const int col = ((int)blockIdx.y * kSumThreads + (threadIdx.x & ((1 << log_group) - 1))) * VE;
+    const int64_t c = (int64_t)blockIdx.x * (kSumThreads >> log_group) + group;
     if (c >= l.stretches || col >= o.dim) return;
     const int64_t lo = c * l.stretch, hi = min(l.n, lo + l.stretch);
-    const uint32_t prev = lo > 0 ? l.keys[lo - 1] : 0xFFFFFFFFu;
-    uint32_t cur = l.keys[lo];
+    uint32_t key[kAhead];
+    Vec<T, VE> next[kAhead];
+    auto fetch = [&](int64_t i0, uint32_t *k, Vec<T, VE> *v) {
+        uint2 e[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) e[j] = i0 + j < hi ? l.pairs[i0 + j] : make_uint2(l.n_nodes, 0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            k[j] = e[j].x;
+            if (k[j] < l.n_nodes) v[j].load_stream(grad + (int64_t)e[j].y * grad_stride + col);
+        }
+    };
+    const uint32_t prev = lo > 0 ? l.key(lo - 1) : 0xFFFFFFFFu, behind = hi < l.n ? l.key(hi) : 0xFFFFFFFFu;
+    const int32_t heads = o.heads != nullptr ? o.heads[c] : 0;
+    fetch(lo, key, next);
+    uint32_t cur = key[0];
     if (cur >= l.n_nodes) return;
     bool open = prev == cur;                   // the id began in a stretch before
-    int32_t seg = o.heads != nullptr ? o.heads[c] - (open ? 1 : 0) : 0;
+    int32_t seg = heads - (open ? 1 : 0);
     float acc[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
     auto flush = [&]() {
-        if (open) {
-            float *p = o.head_part + c * o.dim + col;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) p[i] = acc[i];
-        } else {
-            o.put<VE>(o.heads != nullptr ? seg : (int64_t)cur, col, acc);
-        }
+        if (open) store_part<VE>(o.head_part + c * o.dim + col, acc);
+        else o.put<VE>(o.heads != nullptr ? seg : (int64_t)cur, col, acc);
     };
     auto name = [&]() {
         if (o.unique != nullptr && col == 0 && !open) {
@@ -373,19 +573,20 @@ grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradO
     };
     name();
     for (int64_t i0 = lo; i0 < hi; i0 += kAhead) {
-        uint32_t key[kAhead];
+        uint32_t k[kAhead];
         Vec<T, VE> v[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            key[j] = i0 + j < hi ? l.keys[i0 + j] : l.n_nodes;
-            if (key[j] < l.n_nodes) v[j].load_stream(grad + (int64_t)l.pos[i0 + j] * grad_stride + col);
+            k[j] = key[j];
+            v[j] = next[j];
         }
+        fetch(i0 + kAhead, key, next);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            if (key[j] >= l.n_nodes) continue;  // behind the last entry
-            if (key[j] != cur) {
+            if (k[j] >= l.n_nodes) continue;  // behind the last entry
+            if (k[j] != cur) {
                 flush();
-                cur = key[j];
+                cur = k[j];
                 open = false;
                 ++seg;
                 name();
@@ -396,58 +597,99 @@ grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradO
             for (int i = 0; i < VE; ++i) acc[i] += v[j].get(i);
         }
     }
-    if (hi < l.n && l.keys[hi] == cur) {
-        float *p = o.tail_part + c * o.dim + col;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) p[i] = acc[i];
-    } else {
-        flush();
-    }
+    if (behind == cur) store_part<VE>(o.tail_part + c * o.dim + col, acc);
+    else flush();
 }
 
-// The ids that cross boundaries: the CTA of the stretch where such an id begins adds its pieces, eight threads a column, each
-// every eighth piece, then their eight sums: one fixed order.
-__global__ void __launch_bounds__(256) grad_join_kernel(Sorted l, GradOut o)
+// The ids that cross boundaries: the threads of the stretch where such an id begins add its pieces in list order.  An id of more than
+// kLong pieces is left to the whole CTA: four threads a column, each every fourth piece, then their four sums.
+constexpr int kLong = 24;
+template <int VE>
+__global__ void __launch_bounds__(kSumThreads) grad_join_kernel(Sorted l, GradOut o, int log_group)
 {
-    const int64_t c = blockIdx.x, lo = c * l.stretch, hi = lo + l.stretch;
-    if (hi >= l.n) return;
-    const uint32_t k = l.keys[hi - 1];
-    if (k >= l.n_nodes || l.keys[hi] != k || (lo > 0 && l.keys[lo - 1] == k)) return;
-    int64_t a = hi, b = l.n;   // first entry behind the id
-    while (a < b) {
-        const int64_t m = (a + b) / 2;
-        if (l.keys[m] <= k) a = m + 1;
-        else b = m;
-    }
-    const int64_t last = (a - 1) / l.stretch;
-    const int64_t row = o.heads != nullptr ? o.heads[c + 1] - 1 : (int64_t)k;
-    __shared__ float part[8][32];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int col0 = blockIdx.y * 32; col0 < o.dim; col0 += gridDim.y * 32) {
-        const int col = col0 + x;
-        float acc = 0.0f;
-        if (col < o.dim)
+    __shared__ int32_t longs;
+    __shared__ int64_t long_first[kSumThreads], long_last[kSumThreads];
+    constexpr int kParts = kSumThreads / 32;
+    __shared__ float part[kParts][32 * VE];
+    const int groups = kSumThreads >> log_group;
+    const int in_group = threadIdx.x & ((1 << log_group) - 1);
+    const int col = ((int)blockIdx.y * kSumThreads + in_group) * VE;
+    const int64_t c = (int64_t)blockIdx.x * groups + (threadIdx.x >> log_group), lo = c * l.stretch, hi = lo + l.stretch;
+    if (threadIdx.x == 0) longs = 0;
+    __syncthreads();
+    if (c < l.stretches && hi < l.n) {
+        const uint32_t k = l.key(hi - 1), behind = l.key(hi), before = lo > 0 ? l.key(lo - 1) : 0xFFFFFFFFu;
+        if (k < l.n_nodes && behind == k && before != k) {
+            // the last stretch that begins with the id: c + 1 does; steps that double, then halve
+            int64_t last = c + 1, step = 1;
+            while (last + step < l.stretches && l.key((last + step) * l.stretch) == k) {
+                last += step;
+                step *= 2;
+            }
+            for (; step >= 1; step /= 2)
+                if (last + step < l.stretches && l.key((last + step) * l.stretch) == k) last += step;
+            const int64_t row = o.heads != nullptr ? o.heads[c + 1] - 1 : (int64_t)k;
+            if (last - c >= kLong) {
+                if (in_group == 0) {
+                    const int at = atomicAdd(&longs, 1);   // in which order they are taken changes nothing
+                    long_first[at] = c;
+                    long_last[at] = last;
+                }
+            } else if (col < o.dim) {
+                float acc[VE], v[VE];
+                load_part<VE>(o.tail_part + c * o.dim + col, acc);
 #pragma unroll 4
-            for (int64_t s = c + y; s <= last; s += 8) acc += (s == last ? o.head_part : o.tail_part)[s * o.dim + col];
-        part[y][x] = acc;
-        __syncthreads();
-        if (y == 0 && col < o.dim) {
-            float sum = 0.0f;
+                for (int64_t s = c + 1; s <= last; ++s) {
+                    load_part<VE>((s == last ? o.head_part : o.tail_part) + s * o.dim + col, v);
 #pragma unroll
-            for (int w = 0; w < 8; ++w) sum += part[w][x];
-            o.put<1>(row, col, &sum);
+                    for (int i = 0; i < VE; ++i) acc[i] += v[i];
+                }
+                o.put<VE>(row, col, acc);
+            }
         }
-        __syncthreads();
+    }
+    __syncthreads();
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    for (int q = 0; q < longs; ++q) {
+        const int64_t first = long_first[q], last = long_last[q];
+        const int64_t row = o.heads != nullptr ? o.heads[first + 1] - 1 : (int64_t)l.key((first + 1) * l.stretch);
+        const int end = min(o.dim, ((int)blockIdx.y + 1) * kSumThreads * VE);
+        for (int col0 = (int)blockIdx.y * kSumThreads * VE; col0 < end; col0 += 32 * VE) {
+            const int at = col0 + x * VE;
+            float acc[VE], v[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+            if (at < end)
+#pragma unroll 8
+                for (int64_t s = first + y; s <= last; s += kParts) {
+                    load_part<VE>((s == last ? o.head_part : o.tail_part) + s * o.dim + at, v);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) acc[i] += v[i];
+                }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) part[y][x * VE + i] = acc[i];
+            __syncthreads();
+            if (y == 0 && at < end) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    acc[i] = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kParts; ++w) acc[i] += part[w][x * VE + i];
+                }
+                o.put<VE>(row, at, acc);
+            }
+            __syncthreads();
+        }
     }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 
-static int32_t stretch_of(int64_t n) { return n <= 65536 ? 32 : (n <= 524288 ? 64 : 128); }
+static int32_t stretch_of(int64_t n) { return n <= (1 << 20) ? 32 : (n <= (1 << 22) ? 64 : 128); }
 
 struct GradScratch {
-    uint32_t *keys[2];
-    int32_t *pos[2], *counts, *heads;
+    uint2 *pairs[2];
+    int32_t *counts, *heads;
     float *head_part, *tail_part;
     int64_t bytes;
     GradScratch(uint8_t *base, int64_t n, int64_t dim)
@@ -459,10 +701,7 @@ struct GradScratch {
             return p;
         };
         const int64_t stretches = (n + stretch_of(n) - 1) / stretch_of(n);
-        for (int k = 0; k < 2; ++k) {
-            keys[k] = (uint32_t *)take(4 * n);
-            pos[k] = (int32_t *)take(4 * n);
-        }
+        for (int k = 0; k < 2; ++k) pairs[k] = (uint2 *)take(8 * n);
         counts = (int32_t *)take((int64_t)kSms * kDigits * 4);
         heads = (int32_t *)take(4 * (stretches + 1));
         head_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
@@ -470,80 +709,134 @@ struct GradScratch {
     }
 };
 
-static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch &w, Sorted *l)
+// Most CTAs of a cluster of the sort on the current device: 16 where a group of SMs has that many free, 8 anywhere.
+static int widest_cluster()
+{
+    static int found[64];   // per device, 0: not asked yet
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+    if (found[dev] == 0) {
+        int most = 8;
+        if (cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cluster_sort_smem(kClusterPart)) == cudaSuccess &&
+            cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 16;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(16);
+            cfg.blockDim = dim3(kClusterThreads);
+            cfg.dynamicSmemBytes = (size_t)cluster_sort_smem(kClusterPart);
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            if (cudaOccupancyMaxActiveClusters(&clusters, cluster_sort_kernel, &cfg) == cudaSuccess && clusters >= 1) most = 16;
+        }
+        cudaGetLastError();  // what was refused here is no error of the call
+        found[dev] = most;
+    }
+    return found[dev];
+}
+
+static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch &w, int32_t *count, const ZeroFill &fill, Sorted *l)
 {
     l->n = n;
     l->n_nodes = (uint32_t)ids.n_nodes;
     l->stretch = stretch_of(n);
     l->stretches = (n + l->stretch - 1) / l->stretch;
-    if (n <= kRankMax) {
-        rank_sort_kernel<<<(unsigned)((n + 63) / 64), 256, 0, s>>>(ids, (int)n, w.keys[0], w.pos[0]);
-        l->keys = w.keys[0];
-        l->pos = w.pos[0];
-        LG_LAUNCH_CHECK();
-        return LEGION_OK;
-    }
     int bits = 0;
     while ((ids.n_nodes >> bits) != 0) ++bits;  // n_nodes itself is a key
+    const int widest = widest_cluster();
+    if (n <= (int64_t)widest * kClusterPart) {
+        int ctas = 1;
+        while (ctas < widest && (int64_t)ctas * kClusterThreads < n) ctas *= 2;
+        const int64_t part = ((n + ctas - 1) / ctas + kClusterThreads - 1) / kClusterThreads * kClusterThreads;
+        ClusterSort p{ ids, (int32_t)n, (int32_t)part, FastDiv((uint32_t)part), bits, w.pairs[0], count != nullptr ? w.heads : nullptr, count, l->stretch, fill };
+        // a CTA that fills has 128 KB or more to write; no more of them than surely run at one time beside the sort (clusters of 16 fit
+        // once into each of eight groups of SMs)
+        int64_t fillers = fill.p != nullptr ? (fill.rows * fill.width + (128 << 10) - 1) / (128 << 10) : 0;
+        if (fillers > 112) fillers = 112;
+        fillers = (fillers + ctas - 1) / ctas * ctas;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)ctas;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(ctas + fillers));
+        cfg.blockDim = dim3(kClusterThreads);
+        cfg.dynamicSmemBytes = (size_t)cluster_sort_smem(part);
+        cfg.stream = s;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        LG_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel, p));
+        l->pairs = w.pairs[0];
+        return LEGION_OK;
+    }
+    if (fill.p != nullptr) {
+        if (fill.pitch == fill.width) LG_CUDA(cudaMemsetAsync(fill.p, 0, (size_t)(fill.rows * fill.width), s));
+        else LG_CUDA(cudaMemset2DAsync(fill.p, (size_t)fill.pitch, 0, (size_t)fill.width, (size_t)fill.rows, s));
+    }
     SortPass p;
     p.ids = ids;
     p.counts = w.counts;
     p.n = n;
-    const int64_t ctas = (n + 1023) / 1024 < kSms ? (n + 1023) / 1024 : kSms;
+    const int64_t ctas = kSms;
     p.part = (n + ctas - 1) / ctas;
     int to = 0;
     for (p.shift = 0; p.shift < bits; p.shift += 8, to ^= 1) {
-        p.keys_in = p.shift == 0 ? nullptr : w.keys[to ^ 1];
-        p.pos_in = p.shift == 0 ? nullptr : w.pos[to ^ 1];
-        p.keys_out = w.keys[to];
-        p.pos_out = w.pos[to];
+        p.in = p.shift == 0 ? nullptr : w.pairs[to ^ 1];
+        p.out = w.pairs[to];
         sort_count_kernel<<<(unsigned)ctas, 1024, 0, s>>>(p);
         sort_scatter_kernel<<<(unsigned)ctas, 1024, 0, s>>>(p);
     }
-    l->keys = w.keys[to ^ 1];
-    l->pos = w.pos[to ^ 1];
+    l->pairs = w.pairs[to ^ 1];
+    if (count != nullptr) {
+        head_count_kernel<<<(unsigned)((l->stretches + 7) / 8), 256, 0, s>>>(*l, w.heads);
+        head_scan_kernel<<<1, 1024, 0, s>>>(w.heads, l->stretches, count);
+    }
     LG_LAUNCH_CHECK();
     return LEGION_OK;
 }
 
-template <typename T>
-static void launch_sum(int ve, cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
+template <typename T, int VE>
+static void launch_sum(cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
 {
-    const int vecs = o.dim / ve;
+    const int vecs = o.dim / VE;
     int log_group = 0;
-    while (log_group < 8 && (1 << log_group) < vecs) ++log_group;
-    const int64_t per = 256 >> log_group;
-    const dim3 grid((unsigned)((l.stretches + per - 1) / per), (unsigned)((vecs + 255) / 256));
+    while ((1 << log_group) < kSumThreads && (1 << log_group) < vecs) ++log_group;
+    const int64_t per = kSumThreads >> log_group;
+    const dim3 grid((unsigned)((l.stretches + per - 1) / per), (unsigned)((vecs + kSumThreads - 1) / kSumThreads));
+    grad_sum_kernel<T, VE><<<grid, kSumThreads, 0, s>>>(l, (const T *)grad, stride, o, log_group);
+    if (l.stretches > 1) grad_join_kernel<VE><<<grid, kSumThreads, 0, s>>>(l, o, log_group);
+}
+
+template <typename T>
+static void launch_sum_ve(int ve, cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
+{
     switch (ve) {
     case 8:
-        if constexpr (sizeof(T) == 2) { grad_sum_kernel<T, 8><<<grid, 256, 0, s>>>(l, (const T *)grad, stride, o, log_group); break; }
-    case 4: grad_sum_kernel<T, 4><<<grid, 256, 0, s>>>(l, (const T *)grad, stride, o, log_group); break;
-    case 2: grad_sum_kernel<T, 2><<<grid, 256, 0, s>>>(l, (const T *)grad, stride, o, log_group); break;
-    default: grad_sum_kernel<T, 1><<<grid, 256, 0, s>>>(l, (const T *)grad, stride, o, log_group); break;
+        if constexpr (sizeof(T) == 2) { launch_sum<T, 8>(s, l, grad, stride, o); break; }
+    case 4: launch_sum<T, 4>(s, l, grad, stride, o); break;
+    case 2: launch_sum<T, 2>(s, l, grad, stride, o); break;
+    default: launch_sum<T, 1>(s, l, grad, stride, o); break;
     }
 }
 
 static int run_grad(cudaStream_t s, const Ids &ids, int64_t n, const void *grad, int32_t grad_dtype, int64_t grad_stride, GradOut o,
-                    const GradScratch &w, int32_t *count)
+                    const GradScratch &w, int32_t *count, const ZeroFill &fill)
 {
     Sorted l;
-    int rc = sort_ids(s, ids, n, w, &l);
+    int rc = sort_ids(s, ids, n, w, count, fill, &l);
     if (rc != LEGION_OK) return rc;
     o.head_part = w.head_part;
     o.tail_part = w.tail_part;
-    if (count != nullptr) {
-        head_count_kernel<<<(unsigned)((l.stretches + 7) / 8), 256, 0, s>>>(l, w.heads);
-        head_scan_kernel<<<1, 1024, 0, s>>>(w.heads, l.stretches, count);
-        o.heads = w.heads;
-    }
+    o.heads = count != nullptr ? w.heads : nullptr;
     // what a vector may have: the loads of the gradient are at most 16 bytes, and every address is a multiple of it
     const int ve = common_vector(grad_dtype == LEGION_F32 ? 4 : 8,
                                  { o.dim, grad_stride, aligned_elements(grad, grad_dtype), o.stride, aligned_elements(o.rows, o.dtype) });
-    if (grad_dtype == LEGION_F32) launch_sum<float>(ve, s, l, grad, grad_stride, o);
-    else if (grad_dtype == LEGION_F16) launch_sum<__half>(ve, s, l, grad, grad_stride, o);
-    else launch_sum<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
-    if (l.stretches > 1)
-        grad_join_kernel<<<dim3((unsigned)l.stretches, (unsigned)(o.dim < 512 ? 1 : (o.dim / 512 > 16 ? 16 : o.dim / 512))), 256, 0, s>>>(l, o);
+    if (grad_dtype == LEGION_F32) launch_sum_ve<float>(ve, s, l, grad, grad_stride, o);
+    else if (grad_dtype == LEGION_F16) launch_sum_ve<__half>(ve, s, l, grad, grad_stride, o);
+    else launch_sum_ve<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
     LG_LAUNCH_CHECK();
     return LEGION_OK;
 }
@@ -623,12 +916,12 @@ extern "C" int legion_embedding_grad(int32_t dev_id, const void *ids, int32_t id
     const OnDevice on(dev_id);
     LG_CUDA(on.err);
     cudaStream_t s = (cudaStream_t)stream;
-    const size_t width = (size_t)dim * dtype_bytes(table_dtype);
-    if (!accumulate) {
-        if (table_stride == dim) LG_CUDA(cudaMemsetAsync(grad_table, 0, width * (size_t)n_nodes, s));
-        else LG_CUDA(cudaMemset2DAsync(grad_table, (size_t)table_stride * dtype_bytes(table_dtype), 0, width, (size_t)n_nodes, s));
+    const int64_t width = (int64_t)dim * dtype_bytes(table_dtype), pitch = table_stride * dtype_bytes(table_dtype);
+    if (n_ids == 0) {
+        if (!accumulate) LG_CUDA(cudaMemset2DAsync(grad_table, (size_t)pitch, 0, (size_t)width, (size_t)n_nodes, s));
+        return LEGION_OK;
     }
-    if (n_ids == 0) return LEGION_OK;
+    const ZeroFill fill{ accumulate ? nullptr : (uint8_t *)grad_table, n_nodes, width, pitch };
     GradOut o{};
     o.rows = grad_table;
     o.stride = table_stride;
@@ -636,7 +929,7 @@ extern "C" int legion_embedding_grad(int32_t dev_id, const void *ids, int32_t id
     o.accumulate = accumulate != 0;
     o.scale = scale;
     o.dim = dim;
-    return run_grad(s, Ids{ ids, id_bytes == 8, n_nodes }, n_ids, grad_out, grad_dtype, grad_stride, o, w, nullptr);
+    return run_grad(s, Ids{ ids, id_bytes == 8, n_nodes }, n_ids, grad_out, grad_dtype, grad_stride, o, w, nullptr, fill);
 }
 
 extern "C" int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32_t id_bytes, int64_t n_ids, const void *grad_out,
@@ -667,5 +960,5 @@ extern "C" int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32
     o.wide = id_bytes == 8;
     o.scale = scale;
     o.dim = dim;
-    return run_grad(s, Ids{ ids, id_bytes == 8, n_nodes }, n_ids, grad_out, grad_dtype, grad_stride, o, w, count);
+    return run_grad(s, Ids{ ids, id_bytes == 8, n_nodes }, n_ids, grad_out, grad_dtype, grad_stride, o, w, count, ZeroFill{});
 }

@@ -106,7 +106,8 @@ def test_lookup_far_row_offsets():
 
 SHAPES = [(1, 1, 1, 1.0), (2, 5, 3, 1.0), (31, 40, 64, 2.0), (32, 3, 8, 1.0), (33, 1, 20, 1.0), (333, 5003, 602, 2.0), (1000, 300, 75, 3.0),
           (4096, 2, 100, 1.0), (8192, 700, 16, 2.0), (8193, 700, 16, 2.0), (20000, 40000, 33, 3.0), (70001, 1 << 20, 24, 3.0),
-          (3000, 1 << 24, 4, 2.0)]
+          (3000, 1 << 24, 4, 2.0), (1024, 65535, 12, 1.0), (1025, 65536, 12, 1.0), (90113, 255, 8, 1.0), (180224, 256, 5, 2.0),
+          (180225, 4000, 6, 2.0), (600001, 70000, 4, 3.0)]
 
 
 @pytest.mark.parametrize("n,nodes,dim,skew", SHAPES)
