@@ -683,6 +683,163 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(Sorted l, GradOu
     }
 }
 
+// ---- short lists -----------------------------------------------------------------------------------------------------
+
+constexpr int kDirectMax = 1024;   // lists up to here are not sorted
+constexpr int kDirectThreads = 128;
+constexpr int kFillRows = 32768;   // rows whose presence a CTA notes at a time
+
+// Which positions of the list are the first of their id (a bit each), and how many there are.  One CTA, a thread a position.
+__global__ void __launch_bounds__(kDirectMax) direct_first_kernel(Ids ids, int n, uint32_t *first, int32_t *count)
+{
+    __shared__ uint32_t key[kDirectMax];
+    __shared__ int32_t found[32];
+    const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
+    const uint32_t mine = i < n ? ids.key(i) : (uint32_t)ids.n_nodes;
+    key[i] = mine;
+    __syncthreads();
+    bool is_first = mine < (uint32_t)ids.n_nodes;
+    const uint4 *four = reinterpret_cast<const uint4 *>(key);
+    const int whole = (warp * 32) / 4;   // the positions before this warp's
+    bool seen = false;
+#pragma unroll 8
+    for (int j = 0; j < whole; ++j) {
+        const uint4 k = four[j];
+        seen |= k.x == mine || k.y == mine || k.z == mine || k.w == mine;
+    }
+    const unsigned same = __match_any_sync(kFull, mine);
+    is_first = is_first && !seen && (same & ((1u << lane) - 1u)) == 0;
+    const unsigned all = __ballot_sync(kFull, is_first);
+    if (lane == 0) {
+        first[warp] = all;
+        found[warp] = __popc(all);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int sum = __reduce_add_sync(kFull, found[lane]);
+        if (lane == 0) count[0] = sum;
+    }
+}
+
+// The whole gradient of a list of at most kDirectMax ids without sorting it.  The CTAs of a position read all ids; the position that is
+// the first of its id has the positions of that id in order, and its CTAs add their rows.  Rows of the table that no id names are
+// zeroed by the CTAs behind them, which read all ids too.  n^2 comparisons, but one launch (two for the rows that occur, whose places
+// need the first positions of all ids).
+struct Direct {
+    Ids ids;
+    int32_t n, blocks_y;     // CTAs per position
+    const uint32_t *first;   // rows that occur: direct_first_kernel's bits
+    ZeroFill fill;
+    int32_t fill_word;       // bytes that are zeroed at a time: 16, 4 or 2; every row, start and pitch is a multiple
+    FastDiv words;           // of them in a row
+};
+
+template <typename W>
+__device__ __forceinline__ void zero_absent(const Direct &d, int64_t row0, int rows, const uint32_t *present)
+{
+    W zero = W();
+    const uint32_t all = (uint32_t)rows * d.words.d;   // kFillRows rows have less than 2^32 words
+    uint8_t *base = d.fill.p + row0 * d.fill.pitch;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < all; i += kDirectThreads) {
+        const uint32_t r = d.words.div(i);
+        if ((present[r >> 5] >> (r & 31) & 1u) == 0) reinterpret_cast<W *>(base + (int64_t)r * d.fill.pitch)[i - r * d.words.d] = zero;
+    }
+}
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(kDirectThreads) direct_grad_kernel(Direct d, const T *__restrict__ grad, int64_t grad_stride, GradOut o)
+{
+    __shared__ uint32_t words[kFillRows / 32];   // fill: rows that occur; sums: the positions of the id, 16 bits each
+    __shared__ int32_t counts[kDirectThreads / 32], smaller;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t none = (uint32_t)d.ids.n_nodes;
+    const int position_ctas = d.n * d.blocks_y;
+    if ((int)blockIdx.x >= position_ctas) {
+        const int64_t me = blockIdx.x - position_ctas, ctas = gridDim.x - position_ctas;
+        const int64_t end = d.fill.rows * (me + 1) / ctas;
+        for (int64_t row0 = d.fill.rows * me / ctas; row0 < end; row0 += kFillRows) {
+            const int rows = (int)min((int64_t)kFillRows, end - row0);
+            __syncthreads();
+            for (int i = threadIdx.x; i < (rows + 31) / 32; i += kDirectThreads) words[i] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < d.n; i += kDirectThreads) {
+                const int64_t r = (int64_t)d.ids.key(i) - row0;
+                if (r >= 0 && r < rows) atomicOr(&words[r >> 5], 1u << (r & 31));
+            }
+            __syncthreads();
+            if (d.fill_word == 16) zero_absent<uint4>(d, row0, rows, words);
+            else if (d.fill_word == 4) zero_absent<uint32_t>(d, row0, rows, words);
+            else zero_absent<uint16_t>(d, row0, rows, words);
+        }
+        return;
+    }
+    const int me = blockIdx.x / d.blocks_y, block_y = blockIdx.x - me * d.blocks_y;
+    const uint32_t mine = d.ids.key(me);
+    if (mine >= none) return;
+    uint16_t *list = reinterpret_cast<uint16_t *>(words);
+    if (threadIdx.x == 0) smaller = 0;
+    int found = 0;
+    bool is_first = true;
+    // a warp has a contiguous quarter of the list, so that the positions come in order
+    const int part = ((d.n + kDirectThreads - 1) / kDirectThreads) * 32;
+    uint32_t key[kDirectMax / kDirectThreads];
+#pragma unroll
+    for (int q = 0; q < kDirectMax / kDirectThreads; ++q) {
+        const int i = warp * part + q * 32 + lane;
+        key[q] = q * 32 < part && i < d.n ? d.ids.key(i) : none;
+    }
+    int below = 0;
+#pragma unroll
+    for (int q = 0; q < kDirectMax / kDirectThreads; ++q) {
+        const int i0 = warp * part + q * 32;
+        const unsigned same = __ballot_sync(kFull, key[q] == mine);
+        found += __popc(same);
+        if (same != 0 && i0 + __ffs((int)same) - 1 < me) is_first = false;
+        if (d.first != nullptr && q * 32 < part && i0 < d.n) below += __popc(d.first[i0 >> 5] & __ballot_sync(kFull, key[q] < mine));
+    }
+    if (lane == 0) counts[warp] = found;
+    if (__syncthreads_or(!is_first)) return;
+    if (lane == 0 && below != 0) atomicAdd(&smaller, below);
+    int total = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < kDirectThreads / 32; ++w) {
+        at += w < warp ? counts[w] : 0;
+        total += counts[w];
+    }
+#pragma unroll
+    for (int q = 0; q < kDirectMax / kDirectThreads; ++q) {
+        const unsigned same = __ballot_sync(kFull, key[q] == mine);
+        if (key[q] == mine) list[at + __popc(same & ((1u << lane) - 1u))] = (uint16_t)(warp * part + q * 32 + lane);
+        at += __popc(same);
+    }
+    __syncthreads();
+    const int col = (block_y * kDirectThreads + (int)threadIdx.x) * VE;
+    const int64_t row = d.first != nullptr ? smaller : (int64_t)mine;
+    if (d.first != nullptr && col == 0) {
+        if (o.wide) static_cast<int64_t *>(o.unique)[row] = mine;
+        else static_cast<int32_t *>(o.unique)[row] = (int32_t)mine;
+    }
+    if (col >= o.dim) return;
+    constexpr int kAhead = 8;
+    float acc[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+    for (int j0 = 0; j0 < total; j0 += kAhead) {
+        Vec<T, VE> v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j0 + j < total) v[j].load_stream(grad + (int64_t)list[j0 + j] * grad_stride + col);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j0 + j < total) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) acc[i] += v[j].get(i);
+            }
+    }
+    o.put<VE>(row, col, acc);
+}
+
 // ---- host side -----------------------------------------------------------------------------------------------------
 
 static int32_t stretch_of(int64_t n) { return n <= (1 << 20) ? 32 : (n <= (1 << 22) ? 64 : 128); }
@@ -703,7 +860,7 @@ struct GradScratch {
         const int64_t stretches = (n + stretch_of(n) - 1) / stretch_of(n);
         for (int k = 0; k < 2; ++k) pairs[k] = (uint2 *)take(8 * n);
         counts = (int32_t *)take((int64_t)kSms * kDigits * 4);
-        heads = (int32_t *)take(4 * (stretches + 1));
+        heads = (int32_t *)take(n <= kDirectMax ? kDirectMax / 8 : 4 * (stretches + 1));
         head_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
         tail_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
     }
@@ -810,6 +967,29 @@ static void launch_sum(cudaStream_t s, const Sorted &l, const void *grad, int64_
     if (l.stretches > 1) grad_join_kernel<VE><<<grid, kSumThreads, 0, s>>>(l, o, log_group);
 }
 
+template <typename T, int VE>
+static void launch_direct(cudaStream_t s, Direct d, const void *grad, int64_t stride, const GradOut &o)
+{
+    d.blocks_y = (o.dim / VE + kDirectThreads - 1) / kDirectThreads;
+    // a CTA that fills has 8 KB or more to write
+    int64_t fillers = d.fill.p != nullptr ? (d.fill.rows * d.fill.width + (8 << 10) - 1) / (8 << 10) : 0;
+    if (fillers > d.fill.rows) fillers = d.fill.rows;
+    if (fillers > 16 * kSms) fillers = 16 * kSms;
+    direct_grad_kernel<T, VE><<<(unsigned)(d.n * d.blocks_y + fillers), kDirectThreads, 0, s>>>(d, (const T *)grad, stride, o);
+}
+
+template <typename T>
+static void launch_direct_ve(int ve, cudaStream_t s, const Direct &d, const void *grad, int64_t stride, const GradOut &o)
+{
+    switch (ve) {
+    case 8:
+        if constexpr (sizeof(T) == 2) { launch_direct<T, 8>(s, d, grad, stride, o); break; }
+    case 4: launch_direct<T, 4>(s, d, grad, stride, o); break;
+    case 2: launch_direct<T, 2>(s, d, grad, stride, o); break;
+    default: launch_direct<T, 1>(s, d, grad, stride, o); break;
+    }
+}
+
 template <typename T>
 static void launch_sum_ve(int ve, cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
 {
@@ -825,15 +1005,27 @@ static void launch_sum_ve(int ve, cudaStream_t s, const Sorted &l, const void *g
 static int run_grad(cudaStream_t s, const Ids &ids, int64_t n, const void *grad, int32_t grad_dtype, int64_t grad_stride, GradOut o,
                     const GradScratch &w, int32_t *count, const ZeroFill &fill)
 {
+    // what a vector may have: the loads of the gradient are at most 16 bytes, and every address is a multiple of it
+    const int ve = common_vector(grad_dtype == LEGION_F32 ? 4 : 8,
+                                 { o.dim, grad_stride, aligned_elements(grad, grad_dtype), o.stride, aligned_elements(o.rows, o.dtype) });
+    if (n <= kDirectMax) {
+        int word = 16;
+        while (word > 2 && (fill.width % word != 0 || fill.pitch % word != 0 || (uintptr_t)fill.p % word != 0)) word = word == 16 ? 4 : 2;
+        uint32_t *first = count != nullptr ? (uint32_t *)w.heads : nullptr;
+        const Direct d{ ids, (int32_t)n, 1, first, fill, word, FastDiv((uint32_t)(fill.p != nullptr ? fill.width / word : 1)) };
+        if (count != nullptr) direct_first_kernel<<<1, kDirectMax, 0, s>>>(ids, (int)n, first, count);
+        if (grad_dtype == LEGION_F32) launch_direct_ve<float>(ve, s, d, grad, grad_stride, o);
+        else if (grad_dtype == LEGION_F16) launch_direct_ve<__half>(ve, s, d, grad, grad_stride, o);
+        else launch_direct_ve<__nv_bfloat16>(ve, s, d, grad, grad_stride, o);
+        LG_LAUNCH_CHECK();
+        return LEGION_OK;
+    }
     Sorted l;
     int rc = sort_ids(s, ids, n, w, count, fill, &l);
     if (rc != LEGION_OK) return rc;
     o.head_part = w.head_part;
     o.tail_part = w.tail_part;
     o.heads = count != nullptr ? w.heads : nullptr;
-    // what a vector may have: the loads of the gradient are at most 16 bytes, and every address is a multiple of it
-    const int ve = common_vector(grad_dtype == LEGION_F32 ? 4 : 8,
-                                 { o.dim, grad_stride, aligned_elements(grad, grad_dtype), o.stride, aligned_elements(o.rows, o.dtype) });
     if (grad_dtype == LEGION_F32) launch_sum_ve<float>(ve, s, l, grad, grad_stride, o);
     else if (grad_dtype == LEGION_F16) launch_sum_ve<__half>(ve, s, l, grad, grad_stride, o);
     else launch_sum_ve<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
