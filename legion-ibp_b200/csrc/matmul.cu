@@ -44,9 +44,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
     if (bar_try(bar, parity)) return true;
     return bar_wait_long(bar, parity);
 }
+// PAIR: the barrier may be the other CTA's.
+template <int PAIR>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+    if (PAIR == 2)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                     "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    else asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
                  "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
@@ -71,27 +76,42 @@ __device__ __forceinline__ constexpr uint32_t instruction_desc()
 {
     return (CODEC == LEGION_CODEC_INT8 ? (2u << 4 | 1u << 7 | 1u << 10) : 1u << 4) | (uint32_t)(N / 8) << 17 | (uint32_t)(M / 16) << 24;
 }
-template <int CODEC>
+#define LG_MMA(GROUP, KIND)                                                                                                                  \
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n}" ::"r"(d), \
+                 "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory")
+template <int CODEC, int PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add)
 {
-    if (CODEC == LEGION_CODEC_INT8)
-        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-                     "l"(b), "r"(idesc), "r"(add) : "memory");
-    else
-        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-                     "l"(b), "r"(idesc), "r"(add) : "memory");
+    if (CODEC == LEGION_CODEC_INT8 && PAIR == 1) LG_MMA("1", "i8");
+    else if (CODEC == LEGION_CODEC_INT8) LG_MMA("2", "i8");
+    else if (PAIR == 1) LG_MMA("1", "f8f6f4");
+    else LG_MMA("2", "f8f6f4");
 }
+#undef LG_MMA
+// The barrier (PAIR: of both CTAs) is arrived at when the products issued so far are done.
+template <int PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if (PAIR == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Address of a shared variable in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void pair_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t *r);
-template <>
-__device__ __forceinline__ void tmem_load<16>(uint32_t addr, uint32_t *r)
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t *r)
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -113,10 +133,11 @@ struct MatmulParams {
 
 constexpr int kTileP = 128;
 constexpr int kTileK = 128;   // bytes of a row per stage: one swizzle line
-__host__ __device__ constexpr int stages_of(int bq) { return bq >= 256 ? 4 : (bq >= 128 ? 6 : 8); }
-__host__ __device__ constexpr int stage_bytes(int bq) { return (kTileP + bq) * kTileK; }
+// of one CTA: `bq` columns of the tile, `pair` CTAs that hold half of the Q rows each
+__host__ __device__ constexpr int stage_bytes(int bq, int pair) { return (kTileP + bq / pair) * kTileK; }
+__host__ __device__ constexpr int stages_of(int bq, int pair) { return bq / pair >= 256 ? 4 : (bq / pair >= 128 ? 6 : 8); }
 __host__ __device__ constexpr int tmem_columns(int bq) { return 2 * bq < 32 ? 32 : 2 * bq; }
-constexpr int matmul_smem(int bq) { return stages_of(bq) * stage_bytes(bq) + 1024 + 2 * bq * 4 + 256; }
+constexpr int matmul_smem(int bq, int pair) { return stages_of(bq, pair) * stage_bytes(bq, pair) + 1024 + 2 * bq * 4 + 256; }
 
 // Tiles in groups of kGroupP along P, so that the tiles that run together share rows of both operands in L2.
 constexpr int kGroupP = 16;
@@ -132,21 +153,24 @@ __device__ __forceinline__ void tile_at(int64_t t, int tiles_p, int tiles_q, int
 
 // One CTA per SM takes tiles of 128 x BQ in turn.  Warp 4 loads stages of both operands by TMA, warp 5 issues the products into one of
 // two accumulators in TMEM, warps 0 to 3 scale and store the other one meanwhile.
+// PAIR 2: two CTAs take tiles of 256 x BQ together: each loads its 128 rows of P and half of the rows of Q, the first one issues
+// the products of both, each holds and stores the sums of its own rows of P.
 // P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.
-template <int CODEC, int BQ, bool P_OUT_COLUMNS>
+template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
 __global__ void __launch_bounds__(192, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map, MatmulParams m)
 {
-    constexpr int S = stages_of(BQ);
+    constexpr int S = stages_of(BQ, PAIR), kStage = stage_bytes(BQ, PAIR), kPairP = kTileP * PAIR;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float *q_scale = reinterpret_cast<float *>(smem + S * stage_bytes(BQ));   // [2][BQ]
+    float *q_scale = reinterpret_cast<float *>(smem + S * kStage);   // [2][BQ]
     uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * BQ);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
     volatile int32_t *gave_up = reinterpret_cast<volatile int32_t *>(tmem_slot + 1);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles_p = (m.p_n + kTileP - 1) / kTileP, tiles_q = (m.q_n + BQ - 1) / BQ;
+    const uint32_t me = PAIR == 2 ? blockIdx.x & 1 : 0;   // which of the pair
+    const int tiles_p = (m.p_n + kPairP - 1) / kPairP, tiles_q = (m.q_n + BQ - 1) / BQ;
     const int64_t tiles = (int64_t)tiles_p * tiles_q;
     const int blocks_k = (m.k + kTileK - 1) / kTileK;
 
@@ -157,74 +181,87 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
         }
         for (int a = 0; a < 2; ++a) {
             bar_init(acc_full + 8 * a, 1);
-            bar_init(acc_empty + 8 * a, 128);
+            bar_init(acc_empty + 8 * a, 4 * PAIR);   // the warps that store
         }
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 5) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if (PAIR == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     fence_before();
     __syncthreads();
+    if (PAIR == 2) pair_sync();
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 4) {
         if (lane == 0) {
-            int64_t step = 0;
+            const uint32_t full_of_first = PAIR == 2 ? in_first_cta(full) : full;
+            int s = 0;
+            uint32_t round = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int64_t t = blockIdx.x / PAIR; t < tiles && ok; t += gridDim.x / PAIR) {
                 int tp, tq;
                 tile_at(t, tiles_p, tiles_q, tp, tq);
-                for (int kb = 0; kb < blocks_k; ++kb, ++step) {
-                    const int s = (int)(step % S);
-                    const uint32_t round = (uint32_t)(step / S);
+                for (int kb = 0; kb < blocks_k; ++kb) {
                     if (!bar_wait(empty + 8 * s, (round & 1) ^ 1) || *gave_up) { ok = false; break; }
-                    const uint32_t dst = smem_u32(smem + s * stage_bytes(BQ));
-                    bar_expect(full + 8 * s, stage_bytes(BQ));
-                    tma_2d(dst, &p_map, full + 8 * s, kb * kTileK, tp * kTileP);
-                    tma_2d(dst + kTileP * kTileK, &q_map, full + 8 * s, kb * kTileK, tq * BQ);
+                    const uint32_t dst = smem_u32(smem + s * kStage);
+                    if (me == 0) bar_expect(full + 8 * s, kStage * PAIR);   // what both bring
+                    tma_2d<PAIR>(dst, &p_map, full_of_first + 8 * s, kb * kTileK, tp * kPairP + (int)me * kTileP);
+                    tma_2d<PAIR>(dst + kTileP * kTileK, &q_map, full_of_first + 8 * s, kb * kTileK, tq * BQ + (int)me * (BQ / PAIR));
+                    if (++s == S) { s = 0; ++round; }
                 }
             }
-            if (!ok) {  // the copies that are under way land before the CTA's memory goes
+            // the last products have let go of every stage: nothing signals here any more
+            for (int i = 0; i < S && ok; ++i) {
+                ok = bar_wait(empty + 8 * s, (round & 1) ^ 1);
+                if (++s == S) { s = 0; ++round; }
+            }
+            if (!ok) {  // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
                 *gave_up = 1;
-                for (int64_t i = step > S ? step - S : 0; i < step; ++i) bar_wait(full + 8 * (int)(i % S), (uint32_t)(i / S) & 1);
+                for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = instruction_desc<CODEC, kTileP, BQ>();
-            int64_t step = 0;
-            int turn = 0;
+        if (lane == 0 && me == 0) {
+            constexpr uint32_t idesc = instruction_desc<CODEC, kPairP, BQ>();
+            int s = 0, turn = 0;
+            uint32_t round = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++turn) {
+            for (int64_t t = blockIdx.x / PAIR; t < tiles && ok; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
                 if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1) || *gave_up) { ok = false; break; }
                 fence_after();
-                for (int kb = 0; kb < blocks_k; ++kb, ++step) {
-                    const int s = (int)(step % S);
-                    if (!bar_wait(full + 8 * s, (uint32_t)(step / S) & 1) || *gave_up) { ok = false; break; }
+                for (int kb = 0; kb < blocks_k; ++kb) {
+                    if (!bar_wait(full + 8 * s, round & 1) || *gave_up) { ok = false; break; }
                     fence_after();
-                    const uint32_t src = smem_u32(smem + s * stage_bytes(BQ));
+                    const uint32_t src = smem_u32(smem + s * kStage);
                     const uint64_t dp = operand_desc(src), dq = operand_desc(src + kTileP * kTileK);
                     // 32 codes a product; the last block has as many as the rows reach into
                     const int products = min(kTileK / 32, (m.k - kb * kTileK + 31) / 32);
-                    for (int i = 0; i < products; ++i) mma<CODEC>(tmem + a * BQ, dp + 2 * i, dq + 2 * i, idesc, (kb | i) != 0);
-                    mma_commit(empty + 8 * s);
+                    for (int i = 0; i < products; ++i) mma<CODEC, PAIR>(tmem + a * BQ, dp + 2 * i, dq + 2 * i, idesc, (kb | i) != 0);
+                    mma_commit<PAIR>(empty + 8 * s);
+                    if (++s == S) { s = 0; ++round; }
                 }
-                if (ok) mma_commit(acc_full + 8 * a);
+                if (ok) mma_commit<PAIR>(acc_full + 8 * a);
             }
             if (!ok) *gave_up = 1;
         }
     } else {
+        const uint32_t acc_empty_of_first = PAIR == 2 ? in_first_cta(acc_empty) : acc_empty;
         int turn = 0;
-        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++turn) {
+        for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
             int tp, tq;
             tile_at(t, tiles_p, tiles_q, tp, tq);
             const int a = turn & 1;
-            const int p = tp * kTileP + warp * 32 + lane;
+            const int p = tp * kPairP + (int)me * kTileP + warp * 32 + lane;
             float *qs = q_scale + a * BQ;
             for (int i = threadIdx.x; i < BQ; i += 128) {
                 const int q = tq * BQ + i;
@@ -234,10 +271,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1)) *gave_up = 1;
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
-#pragma unroll
+#pragma unroll 2
             for (int c = 0; c < BQ; c += 16) {
                 uint32_t r[16];
-                tmem_load<16>(tmem + ((uint32_t)(warp * 32) << 16) + a * BQ + c, r);
+                tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + a * BQ + c, r);
                 float v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -271,16 +308,22 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 }
             }
             fence_before();
-            bar_arrive(acc_empty + 8 * a);
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty_of_first + 8 * a) : "memory");
+                else bar_arrive(acc_empty + 8 * a);
+            }
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
+    if (PAIR == 2) pair_sync();   // nothing of the other CTA still signals here, and the products that wrote its TMEM are done
     fence_after();
     if (threadIdx.x == 0 && *gave_up) atomicCAS(&g_operator_error, 0, LEGION_E_TIMEOUT);
     if (warp == 5) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_columns(BQ)));
+        if (PAIR == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_columns(BQ)));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_columns(BQ)));
     }
 }
 
@@ -402,17 +445,28 @@ static int make_map(CUtensorMap *map, const void *rows, int64_t n, int64_t strid
     return LEGION_OK;
 }
 
-template <int CODEC, int BQ, bool P_OUT_COLUMNS>
+template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
 static int launch_tiles(cudaStream_t s, const MatmulParams &m)
 {
     CUtensorMap p_map, q_map;
     int rc = make_map(&p_map, m.p_rows, m.p_n, m.p_stride, m.k, kTileP);
-    if (rc == LEGION_OK) rc = make_map(&q_map, m.q_rows, m.q_n, m.q_stride, m.k, BQ);
+    if (rc == LEGION_OK) rc = make_map(&q_map, m.q_rows, m.q_n, m.q_stride, m.k, BQ / PAIR);
     if (rc != LEGION_OK) return rc;
-    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, matmul_smem(BQ)));
-    const int64_t tiles = (int64_t)((m.p_n + kTileP - 1) / kTileP) * ((m.q_n + BQ - 1) / BQ);
-    matmul_kernel<CODEC, BQ, P_OUT_COLUMNS><<<(unsigned)(tiles < kSms ? tiles : kSms), 192, matmul_smem(BQ), s>>>(p_map, q_map, m);
-    LG_LAUNCH_CHECK();
+    constexpr int smem = matmul_smem(BQ, PAIR);
+    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int64_t tiles = (int64_t)((m.p_n + kTileP * PAIR - 1) / (kTileP * PAIR)) * ((m.q_n + BQ - 1) / BQ);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = PAIR;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles < kSms / PAIR ? tiles : kSms / PAIR) * PAIR);
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = PAIR > 1 ? 1 : 0;
+    LG_CUDA(cudaLaunchKernelEx(&cfg, matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, p_map, q_map, m));
     return LEGION_OK;
 }
 
@@ -432,19 +486,20 @@ static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t
         LG_LAUNCH_CHECK();
         return LEGION_OK;
     }
-    if (m <= 16) return launch_tiles<CODEC, 16, true>(s, by_weight);
-    if (m <= 32) return launch_tiles<CODEC, 32, true>(s, by_weight);
-    if (m <= 64) return launch_tiles<CODEC, 64, true>(s, by_weight);
-    if (m <= 128) return launch_tiles<CODEC, 128, true>(s, by_weight);
+    if (m <= 16) return launch_tiles<CODEC, 16, true, 1>(s, by_weight);
+    if (m <= 32) return launch_tiles<CODEC, 32, true, 1>(s, by_weight);
+    if (m <= 64) return launch_tiles<CODEC, 64, true, 1>(s, by_weight);
+    if (m <= 128) return launch_tiles<CODEC, 128, true, 1>(s, by_weight);
     // wide tiles need the fewest bytes per product; narrower ones where they would leave SMs without work
-    const int64_t tiles_p = (m + kTileP - 1) / kTileP;
-    auto cost = [&](int bq) {
-        const int64_t tiles = tiles_p * ((n + bq - 1) / bq);
-        return (tiles + kSms - 1) / kSms * (bq + 96);
+    auto cost = [&](int bp, int bq, int at_once) {
+        const int64_t tiles = ((m + bp - 1) / bp) * ((n + bq - 1) / bq);
+        return (tiles + at_once - 1) / at_once * (bq + 96);
     };
-    if (cost(256) <= cost(128) && cost(256) <= cost(64)) return launch_tiles<CODEC, 256, false>(s, by_row);
-    if (cost(128) <= cost(64)) return launch_tiles<CODEC, 128, false>(s, by_row);
-    return launch_tiles<CODEC, 64, false>(s, by_row);
+    const int64_t c2 = cost(256, 256, kSms / 2), c256 = cost(128, 256, kSms), c128 = cost(128, 128, kSms), c64 = cost(128, 64, kSms);
+    if (c2 <= c256 && c2 <= c128 && c2 <= c64) return launch_tiles<CODEC, 256, false, 2>(s, by_row);
+    if (c256 <= c128 && c256 <= c64) return launch_tiles<CODEC, 256, false, 1>(s, by_row);
+    if (c128 <= c64) return launch_tiles<CODEC, 128, false, 1>(s, by_row);
+    return launch_tiles<CODEC, 64, false, 1>(s, by_row);
 }
 
 }  // namespace legion
