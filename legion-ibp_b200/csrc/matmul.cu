@@ -111,13 +111,31 @@ __device__ __forceinline__ void pair_sync()
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// 32 columns of the warp's 32 lanes; tmem_wait before the registers are read.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+                 "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+}
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t *r)
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// A tile of shared memory to global memory by TMA, in the calling thread's group of copies.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------------
@@ -129,15 +147,21 @@ struct MatmulParams {
     void *out;
     int64_t out_stride;
     int32_t out_dtype;
+    int32_t by_tma;   // the output's rows start on multiples of 16 bytes
 };
 
 constexpr int kTileP = 128;
 constexpr int kTileK = 128;   // bytes of a row per stage: one swizzle line
 // of one CTA: `bq` columns of the tile, `pair` CTAs that hold half of the Q rows each
 __host__ __device__ constexpr int stage_bytes(int bq, int pair) { return (kTileP + bq / pair) * kTileK; }
-__host__ __device__ constexpr int stages_of(int bq, int pair) { return bq / pair >= 256 ? 4 : (bq / pair >= 128 ? 6 : 8); }
+__host__ __device__ constexpr int stages_of(int bq, int pair) { return bq / pair >= 256 ? 4 : (bq / pair >= 128 ? 5 : 7); }
 __host__ __device__ constexpr int tmem_columns(int bq) { return 2 * bq < 32 ? 32 : 2 * bq; }
-constexpr int matmul_smem(int bq, int pair) { return stages_of(bq, pair) * stage_bytes(bq, pair) + 1024 + 2 * bq * 4 + 256; }
+constexpr int kOutBytes = 32 * 128;   // of a warp's 32 rows, 128 bytes each, on their way out
+__host__ __device__ constexpr int out_buffers(int bq, int pair) { return bq / pair >= 256 ? 1 : 2; }   // what is left of the shared memory
+constexpr int matmul_smem(int bq, int pair)
+{
+    return stages_of(bq, pair) * stage_bytes(bq, pair) + 4 * out_buffers(bq, pair) * kOutBytes + 1024 + 2 * bq * 4 + 256;
+}
 
 // Tiles in groups of kGroupP along P, so that the tiles that run together share rows of both operands in L2.
 constexpr int kGroupP = 16;
@@ -151,19 +175,60 @@ __device__ __forceinline__ void tile_at(int64_t t, int tiles_p, int tiles_q, int
     p = g * kGroupP + rest - q * height;
 }
 
+template <int CODEC>
+__device__ __forceinline__ float sum_of(uint32_t r) { return CODEC == LEGION_CODEC_INT8 ? (float)(int32_t)r : __uint_as_float(r); }
+
+// A warp's 32 rows of a tile, scaled, rounded and on their way: 128 bytes of each row at a time.
+template <int CODEC, typename T, int BQ, int BUFFERS>
+__device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *qs, uint8_t *buffer, const CUtensorMap *map, int q0, int p0,
+                                           const MatmulParams &m, uint32_t &copies)
+{
+    constexpr int kCols = 128 / (int)sizeof(T), kPer16 = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    if (p0 >= m.p_n) return;
+#pragma unroll 1
+    for (int c = 0; c < BQ && q0 + c < m.q_n; c += kCols) {
+        uint8_t *row = buffer + (copies++ % BUFFERS) * kOutBytes + lane * 128;
+        uint32_t r[kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; i += 32) tmem_load32(acc + c + i, r + i);
+        // the copy that read this buffer last is done with it
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFFERS - 1) : "memory");
+        __syncwarp();
+        tmem_wait();
+#pragma unroll
+        for (int i = 0; i < kCols; i += kPer16) {
+            float v[kPer16];
+#pragma unroll
+            for (int j = 0; j < kPer16; ++j) v[j] = sum_of<CODEC>(r[i + j]) * ps * qs[c + i + j];
+            Vec<T, kPer16> o;
+            o.set(v);
+            o.store(reinterpret_cast<T *>(row + ((i / kPer16) ^ (lane & 7)) * 16));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tma_store_2d(map, smem_u32(row), q0 + c, p0);
+    }
+}
+
 // One CTA per SM takes tiles of 128 x BQ in turn.  Warp 4 loads stages of both operands by TMA, warp 5 issues the products into one of
 // two accumulators in TMEM, warps 0 to 3 scale and store the other one meanwhile.
 // PAIR 2: two CTAs take tiles of 256 x BQ together: each loads its 128 rows of P and half of the rows of Q, the first one issues
 // the products of both, each holds and stores the sums of its own rows of P.
+// The output leaves by TMA: a warp writes 128 bytes of each of its 32 rows to shared memory (in the swizzle that the store
+// undoes, so that lanes hit different banks); rows that TMA cannot address are stored by the lanes themselves.
 // P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.
 template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
 __global__ void __launch_bounds__(192, 1)
-matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map, MatmulParams m)
+matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map,
+              const __grid_constant__ CUtensorMap out_map, MatmulParams m)
 {
     constexpr int S = stages_of(BQ, PAIR), kStage = stage_bytes(BQ, PAIR), kPairP = kTileP * PAIR;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float *q_scale = reinterpret_cast<float *>(smem + S * kStage);   // [2][BQ]
+    constexpr int kOut = out_buffers(BQ, PAIR);
+    uint8_t *out_smem = smem + S * kStage;                                                   // [warp][buffer]
+    float *q_scale = reinterpret_cast<float *>(out_smem + 4 * kOut * kOutBytes);             // [2][BQ]
     uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * BQ);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
     volatile int32_t *gave_up = reinterpret_cast<volatile int32_t *>(tmem_slot + 1);
@@ -257,6 +322,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     } else {
         const uint32_t acc_empty_of_first = PAIR == 2 ? in_first_cta(acc_empty) : acc_empty;
         int turn = 0;
+        uint32_t copies = 0;
         for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
             int tp, tq;
             tile_at(t, tiles_p, tiles_q, tp, tq);
@@ -271,40 +337,25 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1)) *gave_up = 1;
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
+            if (!P_OUT_COLUMNS && m.by_tma) {
+                const int p0 = p - lane;
+                if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
+                else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
+                else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
+            } else {
 #pragma unroll 2
-            for (int c = 0; c < BQ; c += 16) {
-                uint32_t r[16];
-                tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + a * BQ + c, r);
-                float v[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    v[i] = (CODEC == LEGION_CODEC_INT8 ? (float)(int32_t)r[i] : __uint_as_float(r[i])) * ps * qs[c + i];
-                const int q0 = tq * BQ + c;
-                if (p >= m.p_n || q0 >= m.q_n) continue;
-                if (P_OUT_COLUMNS) {
+                for (int c = 0; c < BQ; c += 16) {
+                    uint32_t r[16];
+                    tmem_load16(acc + c, r);
+                    tmem_wait();
+                    const int q0 = tq * BQ + c;
+                    if (p >= m.p_n) continue;
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (q0 + i < m.q_n) store_any(m.out, m.out_dtype, (int64_t)(q0 + i) * m.out_stride + p, v[i]);
-                } else {
-                    const int64_t at = (int64_t)p * m.out_stride + q0;
-                    uint8_t *dst = static_cast<uint8_t *>(m.out) + at * dtype_bytes(m.out_dtype);
-                    if (q0 + 16 <= m.q_n && (uintptr_t)dst % 16 == 0) {
-                        if (m.out_dtype == LEGION_F32) {
-                            Vec<float, 8> o[2];
-                            o[0].set(v); o[1].set(v + 8);
-                            o[0].store(reinterpret_cast<float *>(dst)); o[1].store(reinterpret_cast<float *>(dst) + 8);
-                        } else if (m.out_dtype == LEGION_F16) {
-                            Vec<__half, 8> o[2];
-                            o[0].set(v); o[1].set(v + 8);
-                            o[0].store(reinterpret_cast<__half *>(dst)); o[1].store(reinterpret_cast<__half *>(dst) + 8);
-                        } else {
-                            Vec<__nv_bfloat16, 8> o[2];
-                            o[0].set(v); o[1].set(v + 8);
-                            o[0].store(reinterpret_cast<__nv_bfloat16 *>(dst)); o[1].store(reinterpret_cast<__nv_bfloat16 *>(dst) + 8);
-                        }
-                    } else {
-                        for (int i = 0; i < 16 && q0 + i < m.q_n; ++i) store_any(m.out, m.out_dtype, at + i, v[i]);
-                    }
+                        if (q0 + i < m.q_n)
+                            store_any(m.out, m.out_dtype, P_OUT_COLUMNS ? (int64_t)(q0 + i) * m.out_stride + p : (int64_t)p * m.out_stride + q0 + i,
+                                      sum_of<CODEC>(r[i]) * ps * qs[c + i]);
                 }
             }
             fence_before();
@@ -314,6 +365,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 else bar_arrive(acc_empty + 8 * a);
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     fence_before();
@@ -445,13 +497,40 @@ static int make_map(CUtensorMap *map, const void *rows, int64_t n, int64_t strid
     return LEGION_OK;
 }
 
+// boxes of 32 rows, 128 bytes of each; what lies outside of the output is not written
+static int make_out_map(CUtensorMap *map, const MatmulParams &m)
+{
+    EncodeTiled encode = encode_tiled();
+    const int bytes = dtype_bytes(m.out_dtype);
+    const cuuint64_t dims[2] = { (cuuint64_t)m.q_n, (cuuint64_t)m.p_n }, strides[1] = { (cuuint64_t)(m.out_stride * bytes) };
+    const cuuint32_t box[2] = { (cuuint32_t)(128 / bytes), 32 }, one[2] = { 1, 1 };
+    const CUtensorMapDataType type = m.out_dtype == LEGION_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : m.out_dtype == LEGION_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = encode(map, type, 2, m.out, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("legion_matmul_rows: no tensor map for an output of %d x %d, rows %lld elements apart (%d)", m.p_n, m.q_n, (long long)m.out_stride, (int)r);
+        return LEGION_E_CUDA;
+    }
+    return LEGION_OK;
+}
+
 template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
-static int launch_tiles(cudaStream_t s, const MatmulParams &m)
+static int launch_tiles(cudaStream_t s, MatmulParams m)
 {
     CUtensorMap p_map, q_map;
     int rc = make_map(&p_map, m.p_rows, m.p_n, m.p_stride, m.k, kTileP);
     if (rc == LEGION_OK) rc = make_map(&q_map, m.q_rows, m.q_n, m.q_stride, m.k, BQ / PAIR);
     if (rc != LEGION_OK) return rc;
+    CUtensorMap out_map;
+    memset(&out_map, 0, sizeof(out_map));
+    if (!P_OUT_COLUMNS) {
+        const int bytes = dtype_bytes(m.out_dtype);
+        m.by_tma = (uintptr_t)m.out % 16 == 0 && m.out_stride * bytes % 16 == 0;
+        if (m.by_tma) rc = make_out_map(&out_map, m);
+        if (rc != LEGION_OK) return rc;
+    }
     constexpr int smem = matmul_smem(BQ, PAIR);
     LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const int64_t tiles = (int64_t)((m.p_n + kTileP * PAIR - 1) / (kTileP * PAIR)) * ((m.q_n + BQ - 1) / BQ);
@@ -466,7 +545,7 @@ static int launch_tiles(cudaStream_t s, const MatmulParams &m)
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = PAIR > 1 ? 1 : 0;
-    LG_CUDA(cudaLaunchKernelEx(&cfg, matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, p_map, q_map, m));
+    LG_CUDA(cudaLaunchKernelEx(&cfg, matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, p_map, q_map, out_map, m));
     return LEGION_OK;
 }
 
@@ -474,8 +553,8 @@ template <int CODEC>
 static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t row_stride, const uint8_t *weights, int64_t n,
                          int64_t weight_stride, int32_t k, void *out, int32_t out_dtype, int64_t out_stride)
 {
-    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype };
-    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype };
+    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0 };
+    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0 };
     if (m <= 8) {
 #define LG_MATVEC(M, R) matvec_kernel<CODEC, M, R><<<(unsigned)((n + 8 * R - 1) / (8 * R)), 256, 0, s>>>(by_weight)
         if (m == 1) LG_MATVEC(1, 2);
