@@ -97,6 +97,13 @@ __device__ __forceinline__ void mma_commit(uint32_t bar)
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool one_lane()
+{
+    uint32_t mine;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(mine));
+    return mine != 0;
+}
 // Address of a shared variable in the pair's first CTA.
 __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr)
 {
@@ -295,27 +302,36 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             }
         }
     } else if (warp == 5) {
-        if (lane == 0 && me == 0) {
+        if (me == 0) {
+            // the whole warp walks through the stages, so that what the products are issued with is uniform; one lane issues
             constexpr uint32_t idesc = instruction_desc<CODEC, kPairP, BQ>();
             int s = 0, turn = 0;
             uint32_t round = 0;
             bool ok = true;
             for (int64_t t = blockIdx.x / PAIR; t < tiles && ok; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
-                if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1) || *gave_up) { ok = false; break; }
+                ok = bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1) && !*gave_up;
+                if (!__all_sync(kFull, ok)) { ok = false; break; }
                 fence_after();
+                const uint32_t acc = tmem + a * BQ;
                 for (int kb = 0; kb < blocks_k; ++kb) {
-                    if (!bar_wait(full + 8 * s, round & 1) || *gave_up) { ok = false; break; }
+                    ok = bar_wait(full + 8 * s, round & 1) && !*gave_up;
+                    if (!__all_sync(kFull, ok)) { ok = false; break; }
                     fence_after();
                     const uint32_t src = smem_u32(smem + s * kStage);
                     const uint64_t dp = operand_desc(src), dq = operand_desc(src + kTileP * kTileK);
-                    // 32 codes a product; the last block has as many as the rows reach into
-                    const int products = min(kTileK / 32, (m.k - kb * kTileK + 31) / 32);
-                    for (int i = 0; i < products; ++i) mma<CODEC, PAIR>(tmem + a * BQ, dp + 2 * i, dq + 2 * i, idesc, (kb | i) != 0);
-                    mma_commit<PAIR>(empty + 8 * s);
+                    const int left = m.k - kb * kTileK;   // 32 codes a product; the last block has as many as the rows reach into
+                    if (one_lane()) {
+                        mma<CODEC, PAIR>(acc, dp, dq, idesc, kb != 0);
+                        if (left > 32) mma<CODEC, PAIR>(acc, dp + 2, dq + 2, idesc, 1);
+                        if (left > 64) mma<CODEC, PAIR>(acc, dp + 4, dq + 4, idesc, 1);
+                        if (left > 96) mma<CODEC, PAIR>(acc, dp + 6, dq + 6, idesc, 1);
+                        mma_commit<PAIR>(empty + 8 * s);
+                        if (kb == blocks_k - 1) mma_commit<PAIR>(acc_full + 8 * a);
+                    }
+                    __syncwarp();
                     if (++s == S) { s = 0; ++round; }
                 }
-                if (ok) mma_commit<PAIR>(acc_full + 8 * a);
             }
             if (!ok) *gave_up = 1;
         }
