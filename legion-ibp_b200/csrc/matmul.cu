@@ -22,27 +22,17 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
+// Waits until the barrier's phase of that parity is over: at most `tries` times 20 microseconds (kTries: two seconds), then false.
+constexpr uint32_t kTries = 100000;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t tries)
 {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+        "TRY:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n @p bra DONE;\n sub.u32 n, n, 1;\n setp.gt.s32 q, n, 0;\n @q bra TRY;\n"
+        "DONE:\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(tries) : "memory");
     return ok != 0;
-}
-// About two seconds, then the wait is given up (false).
-constexpr long long kWaitClocks = 4000000000ll;
-__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity)
-{
-    const long long t0 = clock64();
-    while (!bar_try(bar, parity))
-        if (clock64() - t0 > kWaitClocks) return false;
-    return true;
-}
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
-{
-    if (bar_try(bar, parity)) return true;
-    return bar_wait_long(bar, parity);
 }
 // PAIR: the barrier may be the other CTA's.
 template <int PAIR>
@@ -155,20 +145,19 @@ struct MatmulParams {
     int64_t out_stride;
     int32_t out_dtype;
     int32_t by_tma;   // the output's rows start on multiples of 16 bytes
+    int32_t stages, stage_bytes, q_at;   // of shared memory; where a stage's rows of Q begin
+    int32_t step_p;   // rows of P per CTA and tile: kTileP, or fewer (a multiple of 8) where that gives every SM a tile
 };
 
 constexpr int kTileP = 128;
 constexpr int kTileK = 128;   // bytes of a row per stage: one swizzle line
-// of one CTA: `bq` columns of the tile, `pair` CTAs that hold half of the Q rows each
-__host__ __device__ constexpr int stage_bytes(int bq, int pair) { return (kTileP + bq / pair) * kTileK; }
-__host__ __device__ constexpr int stages_of(int bq, int pair) { return bq / pair >= 256 ? 4 : (bq / pair >= 128 ? 5 : 7); }
+constexpr int kStagesMax = 32;
 __host__ __device__ constexpr int tmem_columns(int bq) { return 2 * bq < 32 ? 32 : 2 * bq; }
 constexpr int kOutBytes = 32 * 128;   // of a warp's 32 rows, 128 bytes each, on their way out
-__host__ __device__ constexpr int out_buffers(int bq, int pair) { return bq / pair >= 256 ? 1 : 2; }   // what is left of the shared memory
-constexpr int matmul_smem(int bq, int pair)
-{
-    return stages_of(bq, pair) * stage_bytes(bq, pair) + 4 * out_buffers(bq, pair) * kOutBytes + 1024 + 2 * bq * 4 + 256;
-}
+__host__ __device__ constexpr int out_buffers(int bq, int pair) { return bq / pair >= 256 ? 1 : 2; }
+constexpr int kSmem = 227 * 1024;
+// What the stages do not take: alignment, the output's buffers, the scales, the barriers.
+__host__ __device__ constexpr int smem_beside_stages(int bq, int pair) { return 1024 + 4 * out_buffers(bq, pair) * kOutBytes + 2 * bq * 4 + 16 * kStagesMax + 64; }
 
 // Tiles in groups of kGroupP along P, so that the tiles that run together share rows of both operands in L2.
 constexpr int kGroupP = 16;
@@ -182,8 +171,40 @@ __device__ __forceinline__ void tile_at(int64_t t, int tiles_p, int tiles_q, int
     p = g * kGroupP + rest - q * height;
 }
 
-template <int CODEC>
-__device__ __forceinline__ float sum_of(uint32_t r) { return CODEC == LEGION_CODEC_INT8 ? (float)(int32_t)r : __uint_as_float(r); }
+// 32 (or, a tile of 16 columns, 16) sums of a lane's row as fp32.
+template <int CODEC, int N>
+__device__ __forceinline__ void load_sums(uint32_t acc, float *v)
+{
+    uint32_t r[N];
+    if (N == 32) tmem_load32(acc, r);
+    else tmem_load16(acc, r);
+    tmem_wait();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = CODEC == LEGION_CODEC_INT8 ? (float)(int32_t)r[i] : __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void store_one(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store_one(__half *p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void store_one(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// A lane's row of the tile (P_OUT_COLUMNS: its column of the output) by plain stores.
+template <int CODEC, typename T, int BQ, bool P_OUT_COLUMNS>
+__device__ __forceinline__ void store_lane(uint32_t acc, float ps, const float *qs, int q0, int p, bool mine, const MatmulParams &m)
+{
+    constexpr int N = BQ < 32 ? BQ : 32;
+#pragma unroll 1
+    for (int c = 0; c < BQ && q0 + c < m.q_n; c += N) {
+        float v[N];
+        load_sums<CODEC, N>(acc + c, v);
+        if (!mine) continue;
+        const int left = m.q_n - q0 - c;
+        T *dst = static_cast<T *>(m.out) + (P_OUT_COLUMNS ? (int64_t)(q0 + c) * m.out_stride + p : (int64_t)p * m.out_stride + q0 + c);
+        const int64_t step = P_OUT_COLUMNS ? m.out_stride : 1;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) store_one(dst + i * step, v[i] * ps * qs[c + i]);
+    }
+}
 
 // A warp's 32 rows of a tile, scaled, rounded and on their way: 128 bytes of each row at a time.
 template <int CODEC, typename T, int BQ, int BUFFERS>
@@ -196,21 +217,21 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
 #pragma unroll 1
     for (int c = 0; c < BQ && q0 + c < m.q_n; c += kCols) {
         uint8_t *row = buffer + (copies++ % BUFFERS) * kOutBytes + lane * 128;
-        uint32_t r[kCols];
-#pragma unroll
-        for (int i = 0; i < kCols; i += 32) tmem_load32(acc + c + i, r + i);
         // the copy that read this buffer last is done with it
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFFERS - 1) : "memory");
         __syncwarp();
-        tmem_wait();
 #pragma unroll
-        for (int i = 0; i < kCols; i += kPer16) {
-            float v[kPer16];
+        for (int half = 0; half < kCols; half += 32) {
+            float v[32];
+            load_sums<CODEC, 32>(acc + c + half, v);
 #pragma unroll
-            for (int j = 0; j < kPer16; ++j) v[j] = sum_of<CODEC>(r[i + j]) * ps * qs[c + i + j];
-            Vec<T, kPer16> o;
-            o.set(v);
-            o.store(reinterpret_cast<T *>(row + ((i / kPer16) ^ (lane & 7)) * 16));
+            for (int i = 0; i < 32; ++i) v[i] *= ps * qs[c + half + i];
+#pragma unroll
+            for (int i = 0; i < 32; i += kPer16) {
+                Vec<T, kPer16> o;
+                o.set(v + i);
+                o.store(reinterpret_cast<T *>(row + (((half + i) / kPer16) ^ (lane & 7)) * 16));
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -224,39 +245,70 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
 // the products of both, each holds and stores the sums of its own rows of P.
 // The output leaves by TMA: a warp writes 128 bytes of each of its 32 rows to shared memory (in the swizzle that the store
 // undoes, so that lanes hit different banks); rows that TMA cannot address are stored by the lanes themselves.
-// P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.
+// P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.  A tile then has step_p rows of P,
+// as many as spread the weights over all SMs.  The products read 128 rows all the same: what lies behind the tile's rows in shared
+// memory reaches nobody's sums but those of rows that are not stored.
 template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
 __global__ void __launch_bounds__(192, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map,
               const __grid_constant__ CUtensorMap out_map, MatmulParams m)
 {
-    constexpr int S = stages_of(BQ, PAIR), kStage = stage_bytes(BQ, PAIR), kPairP = kTileP * PAIR;
+    constexpr int kPairP = kTileP * PAIR;
+    const int S = m.stages, kStage = m.stage_bytes, q_at = m.q_at;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     constexpr int kOut = out_buffers(BQ, PAIR);
     uint8_t *out_smem = smem + S * kStage;                                                   // [warp][buffer]
     float *q_scale = reinterpret_cast<float *>(out_smem + 4 * kOut * kOutBytes);             // [2][BQ]
     uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * BQ);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStagesMax + 4);
     volatile int32_t *gave_up = reinterpret_cast<volatile int32_t *>(tmem_slot + 1);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t me = PAIR == 2 ? blockIdx.x & 1 : 0;   // which of the pair
-    const int tiles_p = (m.p_n + kPairP - 1) / kPairP, tiles_q = (m.q_n + BQ - 1) / BQ;
+    const int step_p = PAIR == 2 || !P_OUT_COLUMNS ? kPairP : m.step_p;
+    const int tiles_p = (m.p_n + step_p - 1) / step_p, tiles_q = (m.q_n + BQ - 1) / BQ;
     const int64_t tiles = (int64_t)tiles_p * tiles_q;
     const int blocks_k = (m.k + kTileK - 1) / kTileK;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) {
-            bar_init(full + 8 * s, 1);
-            bar_init(empty + 8 * s, 1);
+    // the producer's place: tile, block of its rows, stage, how often the stages have been gone through
+    int64_t tile = blockIdx.x / PAIR;
+    int block = 0, stage = 0, tp = 0, tq = 0;
+    uint32_t round = 0;
+    uint32_t full_of_first = full;
+    auto produce = [&]() {   // the whole warp; one lane issues
+        if (block == 0) tile_at(tile, tiles_p, tiles_q, tp, tq);
+        if (one_lane()) {
+            const uint32_t dst = smem_u32(smem + stage * kStage), bar = full_of_first + 8 * stage;
+            if (me == 0) bar_expect(full + 8 * stage, kStage * PAIR);   // what both bring
+            tma_2d<PAIR>(dst, &p_map, bar, block * kTileK, tp * step_p + (int)me * kTileP);
+            tma_2d<PAIR>(dst + q_at, &q_map, bar, block * kTileK, tq * BQ + (int)me * (BQ / PAIR));
         }
-        for (int a = 0; a < 2; ++a) {
-            bar_init(acc_full + 8 * a, 1);
-            bar_init(acc_empty + 8 * a, 4 * PAIR);   // the warps that store
+        __syncwarp();
+        if (++block == blocks_k) {
+            block = 0;
+            tile += gridDim.x / PAIR;
         }
-        *gave_up = 0;
+        if (++stage == S) {
+            stage = 0;
+            ++round;
+        }
+    };
+    if (warp == 4) {
+        if (lane < S) {
+            bar_init(full + 8 * lane, 1);
+            bar_init(empty + 8 * lane, 1);
+        }
+        if (lane < 2) {
+            bar_init(acc_full + 8 * lane, 1);
+            bar_init(acc_empty + 8 * lane, 4 * PAIR);   // the warps that store
+        }
+        if (lane == 0) *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
+        // the first stages are on their way while the rest is set up; a pair waits for the other's barriers first
+        if (PAIR == 1)
+            while (round == 0 && tile < tiles) produce();
     }
     if (warp == 5) {
         if (PAIR == 2) {
@@ -267,6 +319,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         }
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
     if (PAIR == 2) pair_sync();
@@ -274,52 +327,42 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 4) {
-        if (lane == 0) {
-            const uint32_t full_of_first = PAIR == 2 ? in_first_cta(full) : full;
-            int s = 0;
-            uint32_t round = 0;
-            bool ok = true;
-            for (int64_t t = blockIdx.x / PAIR; t < tiles && ok; t += gridDim.x / PAIR) {
-                int tp, tq;
-                tile_at(t, tiles_p, tiles_q, tp, tq);
-                for (int kb = 0; kb < blocks_k; ++kb) {
-                    if (!bar_wait(empty + 8 * s, (round & 1) ^ 1) || *gave_up) { ok = false; break; }
-                    const uint32_t dst = smem_u32(smem + s * kStage);
-                    if (me == 0) bar_expect(full + 8 * s, kStage * PAIR);   // what both bring
-                    tma_2d<PAIR>(dst, &p_map, full_of_first + 8 * s, kb * kTileK, tp * kPairP + (int)me * kTileP);
-                    tma_2d<PAIR>(dst + kTileP * kTileK, &q_map, full_of_first + 8 * s, kb * kTileK, tq * BQ + (int)me * (BQ / PAIR));
-                    if (++s == S) { s = 0; ++round; }
-                }
+        if (PAIR == 2) full_of_first = in_first_cta(full);
+        uint32_t tries = kTries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
+        while (tile < tiles) {
+            if (!bar_wait(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
+            if (__any_sync(kFull, tries == 0)) break;
+            produce();
+        }
+        // the last products have let go of every stage: nothing signals here any more
+        for (int i = 0; i < S; ++i) {
+            if (!bar_wait(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
+            if (++stage == S) {
+                stage = 0;
+                ++round;
             }
-            // the last products have let go of every stage: nothing signals here any more
-            for (int i = 0; i < S && ok; ++i) {
-                ok = bar_wait(empty + 8 * s, (round & 1) ^ 1);
-                if (++s == S) { s = 0; ++round; }
-            }
-            if (!ok) {  // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
-                *gave_up = 1;
-                for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
-            }
+        }
+        if (tries == 0) {  // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
+            *gave_up = 1;
+            for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
         }
     } else if (warp == 5) {
         if (me == 0) {
-            // the whole warp walks through the stages, so that what the products are issued with is uniform; one lane issues
+            // The whole warp walks through the stages and one lane of it issues: what the products are issued with stays uniform
+            // (issued from a lane on a path of its own, four products took 650 clocks, more than the tensor cores need for 256 x 256).
             constexpr uint32_t idesc = instruction_desc<CODEC, kPairP, BQ>();
+            const uint64_t first = operand_desc(smem_u32(smem));
+            const uint32_t stage16 = (uint32_t)kStage >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
             int s = 0, turn = 0;
-            uint32_t round = 0;
-            bool ok = true;
-            for (int64_t t = blockIdx.x / PAIR; t < tiles && ok; t += gridDim.x / PAIR, ++turn) {
+            uint32_t around = 0, tries = kTries;
+            for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
-                ok = bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1) && !*gave_up;
-                if (!__all_sync(kFull, ok)) { ok = false; break; }
+                if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
                 fence_after();
                 const uint32_t acc = tmem + a * BQ;
                 for (int kb = 0; kb < blocks_k; ++kb) {
-                    ok = bar_wait(full + 8 * s, round & 1) && !*gave_up;
-                    if (!__all_sync(kFull, ok)) { ok = false; break; }
-                    fence_after();
-                    const uint32_t src = smem_u32(smem + s * kStage);
-                    const uint64_t dp = operand_desc(src), dq = operand_desc(src + kTileP * kTileK);
+                    if (!bar_wait(full + 8 * s, around & 1, tries)) tries = 0;
+                    const uint64_t dp = first + (uint32_t)s * stage16, dq = dp + q16;
                     const int left = m.k - kb * kTileK;   // 32 codes a product; the last block has as many as the rows reach into
                     if (one_lane()) {
                         mma<CODEC, PAIR>(acc, dp, dq, idesc, kb != 0);
@@ -330,10 +373,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                         if (kb == blocks_k - 1) mma_commit<PAIR>(acc_full + 8 * a);
                     }
                     __syncwarp();
-                    if (++s == S) { s = 0; ++round; }
+                    if (++s == S) {
+                        s = 0;
+                        ++around;
+                    }
                 }
+                if (__any_sync(kFull, tries == 0)) break;
             }
-            if (!ok) *gave_up = 1;
+            if (tries == 0) *gave_up = 1;
         }
     } else {
         const uint32_t acc_empty_of_first = PAIR == 2 ? in_first_cta(acc_empty) : acc_empty;
@@ -343,36 +390,30 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             int tp, tq;
             tile_at(t, tiles_p, tiles_q, tp, tq);
             const int a = turn & 1;
-            const int p = tp * kPairP + (int)me * kTileP + warp * 32 + lane;
+            const int p = tp * step_p + (int)me * kTileP + warp * 32 + lane;
+            const bool mine = p < m.p_n && warp * 32 + lane + (int)me * kTileP < step_p;
             float *qs = q_scale + a * BQ;
             for (int i = threadIdx.x; i < BQ; i += 128) {
                 const int q = tq * BQ + i;
                 qs[i] = q < m.q_n ? *reinterpret_cast<const float *>(m.q_rows + (int64_t)q * m.q_stride + m.k) : 0.0f;
             }
-            const float ps = p < m.p_n ? *reinterpret_cast<const float *>(m.p_rows + (int64_t)p * m.p_stride + m.k) : 0.0f;
-            if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1)) *gave_up = 1;
+            const float ps = mine ? *reinterpret_cast<const float *>(m.p_rows + (int64_t)p * m.p_stride + m.k) : 0.0f;
+            if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1, kTries)) *gave_up = 1;
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
             const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
-            if (!P_OUT_COLUMNS && m.by_tma) {
-                const int p0 = p - lane;
-                if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
-                else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
-                else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, out_smem + warp * kOut * kOutBytes, &out_map, tq * BQ, p0, m, copies);
-            } else {
-#pragma unroll 2
-                for (int c = 0; c < BQ; c += 16) {
-                    uint32_t r[16];
-                    tmem_load16(acc + c, r);
-                    tmem_wait();
-                    const int q0 = tq * BQ + c;
-                    if (p >= m.p_n) continue;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (q0 + i < m.q_n)
-                            store_any(m.out, m.out_dtype, P_OUT_COLUMNS ? (int64_t)(q0 + i) * m.out_stride + p : (int64_t)p * m.out_stride + q0 + i,
-                                      sum_of<CODEC>(r[i]) * ps * qs[c + i]);
+            if constexpr (!P_OUT_COLUMNS) {
+                if (m.by_tma) {
+                    uint8_t *buffer = out_smem + warp * kOut * kOutBytes;
+                    if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
+                    else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
+                    else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
                 }
+            }
+            if (P_OUT_COLUMNS || !m.by_tma) {
+                if (m.out_dtype == LEGION_F32) store_lane<CODEC, float, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
+                else if (m.out_dtype == LEGION_F16) store_lane<CODEC, __half, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
+                else store_lane<CODEC, __nv_bfloat16, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
             }
             fence_before();
             __syncwarp();
@@ -536,7 +577,7 @@ template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
 static int launch_tiles(cudaStream_t s, MatmulParams m)
 {
     CUtensorMap p_map, q_map;
-    int rc = make_map(&p_map, m.p_rows, m.p_n, m.p_stride, m.k, kTileP);
+    int rc = make_map(&p_map, m.p_rows, m.p_n, m.p_stride, m.k, P_OUT_COLUMNS ? m.step_p : kTileP);
     if (rc == LEGION_OK) rc = make_map(&q_map, m.q_rows, m.q_n, m.q_stride, m.k, BQ / PAIR);
     if (rc != LEGION_OK) return rc;
     CUtensorMap out_map;
@@ -547,17 +588,25 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
         if (m.by_tma) rc = make_out_map(&out_map, m);
         if (rc != LEGION_OK) return rc;
     }
-    constexpr int smem = matmul_smem(BQ, PAIR);
-    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const int64_t tiles = (int64_t)((m.p_n + kTileP * PAIR - 1) / (kTileP * PAIR)) * ((m.q_n + BQ - 1) / BQ);
+    // As many stages as there is room for: what is on its way is what hides the latency of memory.
+    m.q_at = m.step_p * kTileK;
+    m.stage_bytes = m.q_at + BQ / PAIR * kTileK;
+    m.stages = (kSmem - smem_beside_stages(BQ, PAIR)) / m.stage_bytes;
+    if (m.stages > kStagesMax) m.stages = kStagesMax;
+    const int step_p = P_OUT_COLUMNS ? m.step_p : kTileP * PAIR;
+    const int64_t tiles = (int64_t)((m.p_n + step_p - 1) / step_p) * ((m.q_n + BQ - 1) / BQ);
+    const int64_t groups = tiles < kSms / PAIR ? tiles : kSms / PAIR, steps = (tiles + groups - 1) / groups * ((m.k + kTileK - 1) / kTileK);
+    if (m.stages > steps) m.stages = (int32_t)steps;
+    const int smem = m.stages * m.stage_bytes + smem_beside_stages(BQ, PAIR);
+    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = PAIR;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles < kSms / PAIR ? tiles : kSms / PAIR) * PAIR);
+    cfg.gridDim = dim3((unsigned)groups * PAIR);
     cfg.blockDim = dim3(192);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = PAIR > 1 ? 1 : 0;
@@ -565,12 +614,19 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
     return LEGION_OK;
 }
 
+// Few rows on the other side: the weights' bytes are what counts, so every SM gets the same number of them.
+static int32_t weights_per_cta(int64_t n)
+{
+    const int64_t rows = ((n + kSms - 1) / kSms + 7) / 8 * 8;
+    return rows < kTileP ? (int32_t)rows : kTileP;
+}
+
 template <int CODEC>
 static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t row_stride, const uint8_t *weights, int64_t n,
                          int64_t weight_stride, int32_t k, void *out, int32_t out_dtype, int64_t out_stride)
 {
-    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0 };
-    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0 };
+    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0, 0, 0, 0, weights_per_cta(n) };
+    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0, 0, 0, 0, kTileP };
     if (m <= 8) {
 #define LG_MATVEC(M, R) matvec_kernel<CODEC, M, R><<<(unsigned)((n + 8 * R - 1) / (8 * R)), 256, 0, s>>>(by_weight)
         if (m == 1) LG_MATVEC(1, 2);
