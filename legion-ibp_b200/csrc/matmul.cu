@@ -152,6 +152,9 @@ struct MatmulParams {
 constexpr int kTileP = 128;
 constexpr int kTileK = 128;   // bytes of a row per stage: one swizzle line
 constexpr int kStagesMax = 32;
+// Blocks of kTileK codes per stage: what a stage costs beside its products (the wait, the commit, the loop: 230 clocks) is more than the
+// products of a narrow tile.
+__host__ __device__ constexpr int blocks_per_stage(int bq, int pair) { return bq / pair >= 128 ? 1 : 2; }
 __host__ __device__ constexpr int tmem_columns(int bq) { return 2 * bq < 32 ? 32 : 2 * bq; }
 constexpr int kOutBytes = 32 * 128;   // of a warp's 32 rows, 128 bytes each, on their way out
 __host__ __device__ constexpr int out_buffers(int bq, int pair) { return bq / pair >= 256 ? 1 : 2; }
@@ -249,12 +252,14 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
 // as many as spread the weights over all SMs.  The products read 128 rows all the same: what lies behind the tile's rows in shared
 // memory reaches nobody's sums but those of rows that are not stored.
 template <int CODEC, int BQ, bool P_OUT_COLUMNS, int PAIR>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(224, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__ CUtensorMap q_map,
               const __grid_constant__ CUtensorMap out_map, MatmulParams m)
 {
     constexpr int kPairP = kTileP * PAIR;
+    constexpr int kSub = blocks_per_stage(BQ, PAIR);
     const int S = m.stages, kStage = m.stage_bytes, q_at = m.q_at;
+    const uint32_t sub_bytes = (uint32_t)kStage / kSub;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     constexpr int kOut = out_buffers(BQ, PAIR);
@@ -279,13 +284,18 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     auto produce = [&]() {   // the whole warp; one lane issues
         if (block == 0) tile_at(tile, tiles_p, tiles_q, tp, tq);
         if (one_lane()) {
-            const uint32_t dst = smem_u32(smem + stage * kStage), bar = full_of_first + 8 * stage;
-            if (me == 0) bar_expect(full + 8 * stage, kStage * PAIR);   // what both bring
-            tma_2d<PAIR>(dst, &p_map, bar, block * kTileK, tp * step_p + (int)me * kTileP);
-            tma_2d<PAIR>(dst + q_at, &q_map, bar, block * kTileK, tq * BQ + (int)me * (BQ / PAIR));
+            uint32_t dst = smem_u32(smem + stage * kStage);
+            const uint32_t bar = full_of_first + 8 * stage;
+            const int subs = min(kSub, blocks_k - block);
+            if (warp == 4 && me == 0) bar_expect(full + 8 * stage, (uint32_t)subs * sub_bytes * PAIR);   // what all bring
+            for (int i = 0; i < subs; ++i, dst += sub_bytes) {
+                if (warp == 4) tma_2d<PAIR>(dst, &p_map, bar, (block + i) * kTileK, tp * step_p + (int)me * kTileP);
+                else tma_2d<PAIR>(dst + q_at, &q_map, bar, (block + i) * kTileK, tq * BQ + (int)me * (BQ / PAIR));
+            }
         }
         __syncwarp();
-        if (++block == blocks_k) {
+        block += kSub;
+        if (block >= blocks_k) {
             block = 0;
             tile += gridDim.x / PAIR;
         }
@@ -306,9 +316,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
         if (lane == 0) *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         __syncwarp();
-        // the first stages are on their way while the rest is set up; a pair waits for the other's barriers first
-        if (PAIR == 1)
-            while (round == 0 && tile < tiles) produce();
     }
     if (warp == 5) {
         if (PAIR == 2) {
@@ -326,7 +333,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 4) {
+    if (warp == 4 || warp == 6) {
         if (PAIR == 2) full_of_first = in_first_cta(full);
         uint32_t tries = kTries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
         while (tile < tiles) {
@@ -352,7 +359,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             // (issued from a lane on a path of its own, four products took 650 clocks, more than the tensor cores need for 256 x 256).
             constexpr uint32_t idesc = instruction_desc<CODEC, kPairP, BQ>();
             const uint64_t first = operand_desc(smem_u32(smem));
-            const uint32_t stage16 = (uint32_t)kStage >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
+            const uint32_t stage16 = (uint32_t)kStage >> 4, sub16 = sub_bytes >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
             int s = 0, turn = 0;
             uint32_t around = 0, tries = kTries;
             for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
@@ -360,17 +367,18 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
                 fence_after();
                 const uint32_t acc = tmem + a * BQ;
-                for (int kb = 0; kb < blocks_k; ++kb) {
+                for (int kb = 0; kb < blocks_k; kb += kSub) {
                     if (!bar_wait(full + 8 * s, around & 1, tries)) tries = 0;
-                    const uint64_t dp = first + (uint32_t)s * stage16, dq = dp + q16;
+                    const uint64_t dp = first + (uint32_t)s * stage16;
                     const int left = m.k - kb * kTileK;   // 32 codes a product; the last block has as many as the rows reach into
                     if (one_lane()) {
-                        mma<CODEC, PAIR>(acc, dp, dq, idesc, kb != 0);
-                        if (left > 32) mma<CODEC, PAIR>(acc, dp + 2, dq + 2, idesc, 1);
-                        if (left > 64) mma<CODEC, PAIR>(acc, dp + 4, dq + 4, idesc, 1);
-                        if (left > 96) mma<CODEC, PAIR>(acc, dp + 6, dq + 6, idesc, 1);
+#pragma unroll
+                        for (int i = 0; i < 4 * kSub; ++i) {
+                            const uint64_t at = dp + (uint32_t)(i / 4) * sub16 + 2 * (i % 4);
+                            if (i == 0 || left > 32 * i) mma<CODEC, PAIR>(acc, at, at + q16, idesc, i > 0 || kb != 0);
+                        }
                         mma_commit<PAIR>(empty + 8 * s);
-                        if (kb == blocks_k - 1) mma_commit<PAIR>(acc_full + 8 * a);
+                        if (kb + kSub >= blocks_k) mma_commit<PAIR>(acc_full + 8 * a);
                     }
                     __syncwarp();
                     if (++s == S) {
@@ -590,12 +598,13 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
     }
     // As many stages as there is room for: what is on its way is what hides the latency of memory.
     m.q_at = m.step_p * kTileK;
-    m.stage_bytes = m.q_at + BQ / PAIR * kTileK;
+    m.stage_bytes = blocks_per_stage(BQ, PAIR) * (m.q_at + BQ / PAIR * kTileK);
     m.stages = (kSmem - smem_beside_stages(BQ, PAIR)) / m.stage_bytes;
     if (m.stages > kStagesMax) m.stages = kStagesMax;
     const int step_p = P_OUT_COLUMNS ? m.step_p : kTileP * PAIR;
     const int64_t tiles = (int64_t)((m.p_n + step_p - 1) / step_p) * ((m.q_n + BQ - 1) / BQ);
-    const int64_t groups = tiles < kSms / PAIR ? tiles : kSms / PAIR, steps = (tiles + groups - 1) / groups * ((m.k + kTileK - 1) / kTileK);
+    const int64_t groups = tiles < kSms / PAIR ? tiles : kSms / PAIR, a_tile = blocks_per_stage(BQ, PAIR) * kTileK,
+                  steps = (tiles + groups - 1) / groups * ((m.k + a_tile - 1) / a_tile);
     if (m.stages > steps) m.stages = (int32_t)steps;
     const int smem = m.stages * m.stage_bytes + smem_beside_stages(BQ, PAIR);
     LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
@@ -605,7 +614,7 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)groups * PAIR);
-    cfg.blockDim = dim3(192);
+    cfg.blockDim = dim3(224);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cfg.attrs = &attr;
