@@ -144,7 +144,7 @@ struct MatmulParams {
     void *out;
     int64_t out_stride;
     int32_t out_dtype;
-    int32_t by_tma;   // the output's rows start on multiples of 16 bytes
+    int32_t aligned;  // the output's rows start on multiples of 16 bytes
     int32_t stages, stage_bytes, q_at;   // of shared memory; where a stage's rows of Q begin
     int32_t step_p;   // rows of P per CTA and tile: kTileP, or fewer (a multiple of 8) where that gives every SM a tile
 };
@@ -239,6 +239,36 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) tma_store_2d(map, smem_u32(row), q0 + c, p0);
+    }
+}
+
+// The same for P_OUT_COLUMNS where the output's rows start on multiples of 16 bytes: 32 x 32 sums change places in shared memory, so
+// that a lane stores 16 bytes of a row of the output (2-byte stores took 66 clocks each: 4000 clocks for 64 rows).
+template <int CODEC, typename T, int BQ>
+__device__ __forceinline__ void store_turned(uint32_t acc, float ps, const float *qs, uint8_t *buffer, int q0, int p0, int valid, const MatmulParams &m)
+{
+    constexpr int N = BQ < 32 ? BQ : 32, kPer16 = 16 / (int)sizeof(T), kPieces = 32 / kPer16;
+    const int lane = threadIdx.x & 31;
+    T *mine = reinterpret_cast<T *>(buffer);
+#pragma unroll 1
+    for (int c = 0; c < BQ && q0 + c < m.q_n; c += N) {
+        float v[N];
+        load_sums<CODEC, N>(acc + c, v);
+        __syncwarp();   // the last turn's values have been read
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_one(mine + i * 32 + lane, v[i] * ps * qs[c + i]);
+        __syncwarp();
+        const int rows = min(N, m.q_n - q0 - c);
+        for (int i = lane; i < rows * kPieces; i += 32) {
+            const int row = i / kPieces, piece = i % kPieces;
+            T *dst = static_cast<T *>(m.out) + (int64_t)(q0 + c + row) * m.out_stride + p0 + piece * kPer16;
+            const T *src = mine + row * 32 + piece * kPer16;
+            if ((piece + 1) * kPer16 <= valid) {
+                *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+            } else {
+                for (int j = 0; j < kPer16 && piece * kPer16 + j < valid; ++j) dst[j] = src[j];
+            }
+        }
     }
 }
 
@@ -410,15 +440,19 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
             const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
-            if constexpr (!P_OUT_COLUMNS) {
-                if (m.by_tma) {
-                    uint8_t *buffer = out_smem + warp * kOut * kOutBytes;
+            uint8_t *buffer = out_smem + warp * kOut * kOutBytes;
+            if (m.aligned && P_OUT_COLUMNS) {
+                const int p0 = p - lane, valid = min(step_p - warp * 32, m.p_n - p0);
+                if (m.out_dtype == LEGION_F32) store_turned<CODEC, float, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
+                else if (m.out_dtype == LEGION_F16) store_turned<CODEC, __half, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
+                else store_turned<CODEC, __nv_bfloat16, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
+            } else if (m.aligned) {
+                if constexpr (!P_OUT_COLUMNS) {
                     if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
                     else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
                     else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
                 }
-            }
-            if (P_OUT_COLUMNS || !m.by_tma) {
+            } else {
                 if (m.out_dtype == LEGION_F32) store_lane<CODEC, float, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
                 else if (m.out_dtype == LEGION_F16) store_lane<CODEC, __half, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
                 else store_lane<CODEC, __nv_bfloat16, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
@@ -590,12 +624,9 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
     if (rc != LEGION_OK) return rc;
     CUtensorMap out_map;
     memset(&out_map, 0, sizeof(out_map));
-    if (!P_OUT_COLUMNS) {
-        const int bytes = dtype_bytes(m.out_dtype);
-        m.by_tma = (uintptr_t)m.out % 16 == 0 && m.out_stride * bytes % 16 == 0;
-        if (m.by_tma) rc = make_out_map(&out_map, m);
-        if (rc != LEGION_OK) return rc;
-    }
+    m.aligned = (uintptr_t)m.out % 16 == 0 && m.out_stride * dtype_bytes(m.out_dtype) % 16 == 0;
+    if (m.aligned && !P_OUT_COLUMNS) rc = make_out_map(&out_map, m);
+    if (rc != LEGION_OK) return rc;
     // As many stages as there is room for: what is on its way is what hides the latency of memory.
     m.q_at = m.step_p * kTileK;
     m.stage_bytes = blocks_per_stage(BQ, PAIR) * (m.q_at + BQ / PAIR * kTileK);
