@@ -403,7 +403,7 @@ def _refused(what, t, dev_id, dims, shape):
 def _operand(what, t, dev_id, dims, shape=None):
     """Type code of a tensor, after the checks that a pointer cannot make: where it lies, its shape, whole rows."""
     s = t.shape
-    if len(s) != dims or (shape is not None and s != shape) or t.get_device() != dev_id or not t.is_cuda or (s[-1] > 1 and t.stride(-1) != 1):
+    if len(s) != dims or (shape is not None and s != shape) or t.get_device() != dev_id or (s[-1] > 1 and t.stride()[-1] != 1):
         raise _refused(what, t, dev_id, dims, shape)
     return _dtypes.get(t.dtype) or _code_of(t.dtype)
 
@@ -411,18 +411,18 @@ def _operand(what, t, dev_id, dims, shape=None):
 def _rows(what, t, dev_id, shape=None):
     """(type code, elements from row to row) of float rows; one row (or none) has no next one."""
     s, step = t.shape, t.stride()
-    if len(s) != 2 or (shape is not None and s != shape) or t.get_device() != dev_id or not t.is_cuda or (s[1] > 1 and step[1] != 1):
+    if len(s) != 2 or (shape is not None and s != shape) or t.get_device() != dev_id or (step[1] != 1 and s[1] > 1):
         raise _refused(what, t, dev_id, 2, shape)
     code = (_dtypes.get(t.dtype) or _code_of(t.dtype))[0]
     if code < 0:
         raise LegionError("%s: %s is not float32, float16 or bfloat16" % (what, t.dtype))
-    n, dim = s
-    return code, step[0] if n > 1 or step[0] >= dim else dim
+    step = step[0]
+    return code, step if step >= s[1] or s[0] > 1 else s[1]
 
 
 def _id_width(what, ids, dev_id):
     code, width = _operand(what, ids, dev_id, 1)
-    if code >= 0 or width not in (4, 8):
+    if width < 4:
         raise LegionError("%s: %s is not int32 or int64" % (what, ids.dtype))
     return width
 
@@ -430,10 +430,12 @@ def _id_width(what, ids, dev_id):
 def _code_rows(what, t, dev_id, feature_len):
     if _operand(what, t, dev_id, 2) != (-1, 1):
         raise LegionError("%s: %s is not uint8" % (what, t.dtype))
-    need = (feature_len + 4 + 15) // 16 * 16
-    if t.shape[1] < need:
-        raise LegionError("%s: rows of %d bytes, compressed rows of %d codes have %d" % (what, t.shape[1], feature_len, need))
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), need) + 15 & -16
+    need = feature_len + 19 & -16
+    n, width = t.shape
+    if width < need:
+        raise LegionError("%s: rows of %d bytes, compressed rows of %d codes have %d" % (what, width, feature_len, need))
+    step = t.stride()[0]
+    return step if n > 1 or step >= need else need
 
 
 def _workspace(t, dev_id):
@@ -445,7 +447,7 @@ def _workspace(t, dev_id):
 
 
 def _handle(stream):
-    return None if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def embedding_lookup(dev_id, table, ids, out, scale=1.0, stream=None):
@@ -455,8 +457,10 @@ def embedding_lookup(dev_id, table, ids, out, scale=1.0, stream=None):
     width = _id_width("ids", ids, dev_id)
     n, (nodes, dim) = ids.shape[0], table.shape
     od, os_ = _rows("out", out, dev_id, (n, dim))
-    _check((_lib or lib()).legion_embedding_lookup(dev_id, table.data_ptr(), td, ts, nodes, ids.data_ptr(), width, n, dim, scale,
-                                                   out.data_ptr(), od, os_, _handle(stream)))
+    rc = (_lib or lib()).legion_embedding_lookup(dev_id, table.data_ptr(), td, ts, nodes, ids.data_ptr(), width, n, dim, scale,
+                                                   out.data_ptr(), od, os_, None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def embedding_grad_workspace(n_ids, dim, n_nodes):
@@ -474,8 +478,10 @@ def embedding_grad(dev_id, ids, grad_out, grad_table, workspace, scale=1.0, accu
     n, (nodes, dim) = ids.shape[0], grad_table.shape
     gd, gs = _rows("grad_out", grad_out, dev_id, (n, dim))
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check((_lib or lib()).legion_embedding_grad(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale,
-                                                 grad_table.data_ptr(), td, ts, nodes, 1 if accumulate else 0, ws, ws_bytes, _handle(stream)))
+    rc = (_lib or lib()).legion_embedding_grad(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale,
+                                                 grad_table.data_ptr(), td, ts, nodes, 1 if accumulate else 0, ws, ws_bytes, None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, count, workspace, scale=1.0, stream=None):
@@ -494,9 +500,11 @@ def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, c
     if _operand("count", count, dev_id, 1, (1,)) != (-1, 4):
         raise LegionError("count must be one int32")
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check((_lib or lib()).legion_embedding_grad_rows(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale, n_nodes,
+    rc = (_lib or lib()).legion_embedding_grad_rows(dev_id, ids.data_ptr(), width, n, grad_out.data_ptr(), gd, gs, dim, scale, n_nodes,
                                                       unique_ids.data_ptr(), grad_rows.data_ptr(), rs, count.data_ptr(), ws, ws_bytes,
-                                                      _handle(stream)))
+                                                      None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def rms_norm(dev_id, x, weight, out, eps=1e-6, residual=None, residual_out=None, codec=CODEC_RAW, stream=None):
@@ -521,8 +529,10 @@ def rms_norm(dev_id, x, weight, out, eps=1e-6, residual=None, residual_out=None,
             raise LegionError("out: %d rows, expected %d" % (out.shape[0], n))
     if rd != dt or td != dt or od != dt:
         raise LegionError("residual, residual_out and out must be of x's type")
-    _check((_lib or lib()).legion_rms_norm(dev_id, x.data_ptr(), dt, xs, rp or None, rs, weight.data_ptr(), wd, eps, n, dim, codec,
-                                           out.data_ptr(), os_, tp or None, ts, _handle(stream)))
+    rc = (_lib or lib()).legion_rms_norm(dev_id, x.data_ptr(), dt, xs, rp or None, rs, weight.data_ptr(), wd, eps, n, dim, codec,
+                                           out.data_ptr(), os_, tp or None, ts, None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def rms_norm_grad_workspace(n_rows, dim):
@@ -547,8 +557,10 @@ def rms_norm_grad(dev_id, grad_out, x, weight, grad_x, grad_weight, workspace, e
         raise LegionError("grad_out, grad_x and grad_residual must be of x's type")
     wd, wg = _operand("weight", weight, dev_id, 1, (dim,))[0], _operand("grad_weight", grad_weight, dev_id, 1, (dim,))[0]
     ws, ws_bytes = _workspace(workspace, dev_id)
-    _check((_lib or lib()).legion_rms_norm_grad(dev_id, grad_out.data_ptr(), gs, x.data_ptr(), xs, dt, rp, rs, weight.data_ptr(), wd, eps, n,
-                                                dim, grad_x.data_ptr(), os_, grad_weight.data_ptr(), wg, ws, ws_bytes, _handle(stream)))
+    rc = (_lib or lib()).legion_rms_norm_grad(dev_id, grad_out.data_ptr(), gs, x.data_ptr(), xs, dt, rp, rs, weight.data_ptr(), wd, eps, n,
+                                                dim, grad_x.data_ptr(), os_, grad_weight.data_ptr(), wg, ws, ws_bytes, None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None):
@@ -557,14 +569,16 @@ def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None)
     rs, ws = _code_rows("rows", rows, dev_id, feature_len), _code_rows("weight_rows", weight_rows, dev_id, feature_len)
     m, n = rows.shape[0], weight_rows.shape[0]
     od, os_ = _rows("out", out, dev_id, (m, n))
-    _check((_lib or lib()).legion_matmul_rows(dev_id, codec, rows.data_ptr(), m, rs, weight_rows.data_ptr(), n, ws, feature_len,
-                                              out.data_ptr(), od, os_, _handle(stream)))
+    rc = (_lib or lib()).legion_matmul_rows(dev_id, codec, rows.data_ptr(), m, rs, weight_rows.data_ptr(), n, ws, feature_len,
+                                              out.data_ptr(), od, os_, None if stream is None else _handle(stream))
+    if rc:
+        _check(rc)
 
 
 def operator_error(dev_id, stream=None, reset=True):
     """First error that a kernel of these operators raised on dev_id since the last reset (0: none)."""
     e = C.c_int32()
-    _check(lib().legion_operator_error(dev_id, _handle(stream), C.byref(e), 1 if reset else 0))
+    _check(lib().legion_operator_error(dev_id, None if stream is None else _handle(stream), C.byref(e), 1 if reset else 0))
     return e.value
 
 

@@ -501,64 +501,51 @@ __device__ __forceinline__ void dot16(const uint4 &a, const uint4 &b, typename s
     }
 }
 
-// A warp has R weight rows and all M rows of the other side: bound by the weights' bytes, each read once.
-template <int CODEC, int M, int R>
+// One row against weight rows that are read once: a warp has R weight rows.  Bound by the weights' bytes, and nearly by __dp4a, which
+// runs once per 7 clocks and SM: 15.7 us by 16384 x 4096, where a plain read of the 67 MB takes 12.9.  (Two rows took 20 us, eight
+// 40: they go to the tensor cores, which take 18 us for up to 16.)
+template <int CODEC, int R>
 __global__ void __launch_bounds__(256) matvec_kernel(MatmulParams m)
 {
     typedef typename std::conditional<CODEC == LEGION_CODEC_INT8, int, float>::type acc_t;
     const int lane = threadIdx.x & 31;
     const int64_t n0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * R;
     if (n0 >= m.p_n) return;
-    acc_t acc[R][M];
+    float ws[R];   // asked for before the codes
+    const float xs = *reinterpret_cast<const float *>(m.q_rows + m.k);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) ws[r] = n0 + r < m.p_n ? *reinterpret_cast<const float *>(m.p_rows + (n0 + r) * m.p_stride + m.k) : 0.0f;
+    acc_t acc[R];
 #pragma unroll
-        for (int i = 0; i < M; ++i) acc[r][i] = 0;
+    for (int r = 0; r < R; ++r) acc[r] = 0;
     const int chunks = m.k / 16;   // whole 16-byte pieces
-#pragma unroll 2
+#pragma unroll 4
     for (int c = lane; c < chunks; c += 32) {
-        uint4 w[R], x[M];
+        uint4 w[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             w[r] = make_uint4(0, 0, 0, 0);
             if (n0 + r < m.p_n) w[r] = __ldcs(reinterpret_cast<const uint4 *>(m.p_rows + (n0 + r) * m.p_stride) + c);
         }
+        const uint4 x = *(reinterpret_cast<const uint4 *>(m.q_rows) + c);
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-            x[i] = make_uint4(0, 0, 0, 0);
-            if (i < m.q_n) x[i] = *(reinterpret_cast<const uint4 *>(m.q_rows + i * m.q_stride) + c);
-        }
+        for (int r = 0; r < R; ++r) dot16<CODEC>(w[r], x, acc[r]);
+    }
+    if (lane < (m.k % 16) / 4) {   // words behind them, one a lane
+        const uint32_t x = reinterpret_cast<const uint32_t *>(m.q_rows)[chunks * 4 + lane];
 #pragma unroll
         for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int i = 0; i < M; ++i) dot16<CODEC>(w[r], x[i], acc[r][i]);
-    }
-    const int rest = (m.k % 16) / 4;   // words behind them, one a lane
-    if (lane < rest) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (n0 + r >= m.p_n) continue;
-            const uint32_t w = reinterpret_cast<const uint32_t *>(m.p_rows + (n0 + r) * m.p_stride)[chunks * 4 + lane];
-#pragma unroll
-            for (int i = 0; i < M; ++i)
-                if (i < m.q_n)
-                    dot16<CODEC>(make_uint4(w, 0, 0, 0),
-                                 make_uint4(reinterpret_cast<const uint32_t *>(m.q_rows + i * m.q_stride)[chunks * 4 + lane], 0, 0, 0), acc[r][i]);
-        }
+            if (n0 + r < m.p_n)
+                dot16<CODEC>(make_uint4(reinterpret_cast<const uint32_t *>(m.p_rows + (n0 + r) * m.p_stride)[chunks * 4 + lane], 0, 0, 0),
+                             make_uint4(x, 0, 0, 0), acc[r]);
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        acc_t a = acc[r];
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-            acc_t a = acc[r][i];
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) a += __shfl_xor_sync(kFull, a, d);
-            if (lane == (r * M + i) % 32 && n0 + r < m.p_n && i < m.q_n) {
-                const float ws = *reinterpret_cast<const float *>(m.p_rows + (n0 + r) * m.p_stride + m.k);
-                const float xs = *reinterpret_cast<const float *>(m.q_rows + i * m.q_stride + m.k);
-                store_any(m.out, m.out_dtype, i * m.out_stride + n0 + r, (float)a * ws * xs);
-            }
-        }
+        for (int d = 16; d > 0; d >>= 1) a += __shfl_xor_sync(kFull, a, d);
+        if (lane == r && n0 + r < m.p_n) store_any(m.out, m.out_dtype, n0 + r, (float)a * ws[r] * xs);
+    }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------
@@ -575,6 +562,18 @@ static EncodeTiled encode_tiled()
             fn = (EncodeTiled)p;
     }
     return fn;
+}
+
+// What a kernel's launch asks for once per device: more than 48 KB of shared memory.
+static int allow_smem(const void *kernel, int bytes, bool *done)
+{
+    int dev = 0;
+    LG_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !done[dev]) {
+        LG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+    return LEGION_OK;
 }
 
 // k codes of n rows; what a box reaches beyond them (the scales among it) arrives as zeros
@@ -638,7 +637,9 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
                   steps = (tiles + groups - 1) / groups * ((m.k + a_tile - 1) / a_tile);
     if (m.stages > steps) m.stages = (int32_t)steps;
     const int smem = m.stages * m.stage_bytes + smem_beside_stages(BQ, PAIR);
-    LG_CUDA(cudaFuncSetAttribute(matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    static bool allowed[64];
+    rc = allow_smem((const void *)matmul_kernel<CODEC, BQ, P_OUT_COLUMNS, PAIR>, kSmem, allowed);
+    if (rc != LEGION_OK) return rc;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = PAIR;
@@ -667,13 +668,8 @@ static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t
 {
     const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0, 0, 0, 0, weights_per_cta(n) };
     const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0, 0, 0, 0, kTileP };
-    if (m <= 8) {
-#define LG_MATVEC(M, R) matvec_kernel<CODEC, M, R><<<(unsigned)((n + 8 * R - 1) / (8 * R)), 256, 0, s>>>(by_weight)
-        if (m == 1) LG_MATVEC(1, 2);
-        else if (m == 2) LG_MATVEC(2, 2);
-        else if (m <= 4) LG_MATVEC(4, 2);
-        else LG_MATVEC(8, 2);
-#undef LG_MATVEC
+    if (m == 1) {
+        matvec_kernel<CODEC, 2><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(by_weight);
         LG_LAUNCH_CHECK();
         return LEGION_OK;
     }

@@ -37,7 +37,7 @@ def _check(got, a, b, k, codec):
     _close(got, want, slack)
 
 
-SHAPES = [(1, 1, 4), (1, 5, 16), (2, 33, 20), (3, 130, 36), (4, 64, 128), (5, 1000, 132), (7, 16, 2048), (8, 17, 1028), (9, 300, 64), (16, 128, 256),
+SHAPES = [(1, 1, 4), (1, 5, 16), (2, 33, 20), (3, 130, 36), (4, 64, 128), (5, 1000, 132), (7, 16, 2048), (1, 700, 4100), (2, 601, 508), (3, 5000, 1036), (6, 9500, 8), (8, 1203, 4108), (4, 4097, 520), (5, 40, 12), (8, 17, 1028), (9, 300, 64), (16, 128, 256),
           (17, 129, 260), (33, 500, 768), (64, 64, 516), (65, 257, 100), (127, 128, 128), (128, 1000, 384), (129, 100, 132), (200, 513, 1024),
           (300, 256, 640), (611, 1000, 768), (1030, 70, 40), (257, 2600, 4096), (5000, 260, 128), (2049, 9001, 260), (4096, 8192, 128), (3000, 9100, 1100)]
 
