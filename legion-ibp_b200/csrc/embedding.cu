@@ -106,6 +106,7 @@ constexpr int kDigits = 256;
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterItems = 11;                            // entries that a thread has at most
 constexpr int kClusterPart = kClusterItems * kClusterThreads; // entries that a CTA has at most
+constexpr int64_t kClusterList = 32768;                      // longest list that a cluster sorts
 constexpr int kHistPitch = kDigits + 1;                      // the 32 counts of a digit lie in 32 banks
 
 // The rows of the gradient that no id names are zeros: the CTAs of the sorting launch that have nothing to sort write them (all
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(Cluste
         zero_fill(p.fill, (int64_t)(blockIdx.x - size) * kClusterThreads + threadIdx.x, (int64_t)(gridDim.x - size) * kClusterThreads);
         return;
     }
+    cudaTriggerProgrammaticLaunchCompletion();
     const uint32_t me = cluster_rank();
     uint2 *buf[2] = { reinterpret_cast<uint2 *>(smem), reinterpret_cast<uint2 *>(smem) + p.part };
     int32_t *hist = reinterpret_cast<int32_t *>(buf[1] + p.part);  // [warp][digit]
@@ -329,88 +331,117 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(Cluste
     cluster_sync();  // no CTA's memory goes while another one may read it
 }
 
-// Lists that no cluster holds: the same passes over global memory, every CTA one contiguous part of the list.
+// Longer lists: the same passes over global memory, every CTA one contiguous part of the list.  A pass is one launch: it reads the counts
+// of all parts' digits, and counts the next pass's digits of the parts that its entries go to (whole numbers: the order of the
+// atomics changes nothing).  What bounds a pass is the chain of latencies in it; the launches are dependents that start while the one
+// before ends.
+constexpr int kPassMax = 4;
 struct SortPass {
     Ids ids;                  // first pass: the ids themselves
     const uint2 *in;          // later ones: the pairs
     uint2 *out;
-    int32_t *counts;          // [CTA][digit]
-    int64_t n, part;          // entries, entries per CTA
+    int32_t *counts;          // [CTA][digit] of this pass
+    int32_t *next;            // of the next one, or nullptr
+    int64_t n;
+    int32_t part;             // entries per CTA
+    FastDiv per_part;
     int32_t shift;
     __device__ __forceinline__ uint2 pair(int64_t i) const { return in != nullptr ? in[i] : make_uint2(ids.key(i), (uint32_t)i); }
 };
 
-__global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p)
+// The first pass's counts; the others' are zeroed.
+__global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p, int passes)
 {
     __shared__ int32_t hist[kDigits];
     if (threadIdx.x < kDigits) hist[threadIdx.x] = 0;
+    for (int q = 1; q < passes; ++q)
+        for (int i = threadIdx.x; i < kDigits; i += blockDim.x) p.counts[(q * kSms + blockIdx.x) * kDigits + i] = 0;
+    cudaTriggerProgrammaticLaunchCompletion();
     __syncthreads();
-    const int64_t lo = blockIdx.x * p.part, hi = min(p.n, lo + p.part);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&hist[(p.pair(i).x >> p.shift) & (kDigits - 1)], 1);
+    const int64_t lo = (int64_t)blockIdx.x * p.part, hi = min(p.n, lo + p.part);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&hist[p.ids.key(i) & (kDigits - 1)], 1);
     __syncthreads();
     if (threadIdx.x < kDigits) p.counts[blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
 {
-    __shared__ int32_t whist[32][kDigits];  // per warp: entries of a digit, then where its first one goes
+    __shared__ int32_t whist[32][kHistPitch];  // per warp: entries of a digit, then where its first one goes
     __shared__ int32_t base[kDigits];
-    __shared__ int32_t warp_sum[8];
+    __shared__ int32_t scan[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int d = threadIdx.x & (kDigits - 1), g = threadIdx.x >> 8;
-    // entries of smaller digits, and of the same digit in the parts before this one
-    int total = 0, before = 0;
-#pragma unroll 8
-    for (int c = g; c < (int)gridDim.x; c += 4) {
-        const int v = p.counts[c * kDigits + d];
-        total += v;
-        before += c < (int)blockIdx.x ? v : 0;
-    }
-    whist[g][d] = total;
-    whist[4 + g][d] = before;
-    __syncthreads();
-    int incl = 0, mine = 0;
-    if (threadIdx.x < kDigits) {
-        mine = whist[0][d] + whist[1][d] + whist[2][d] + whist[3][d];
-        before = whist[4][d] + whist[5][d] + whist[6][d] + whist[7][d];
-        incl = mine;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int v = __shfl_up_sync(kFull, incl, s);
-            if (lane >= s) incl += v;
+    for (int k = threadIdx.x; k < 32 * kHistPitch; k += 1024) (&whist[0][0])[k] = 0;
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int64_t lo = (int64_t)blockIdx.x * p.part, hi = min(p.n, lo + p.part);
+    uint2 e = lo + threadIdx.x < hi ? p.pair(lo + threadIdx.x) : make_uint2(0, 0);
+    {   // entries of smaller digits, and of the same digit in the parts before this one; warp w has digits 8 w to 8 w + 7, a quarter
+        // of the parts per eight lanes
+        const int d = warp * 8 + (lane & 7), g = lane >> 3;
+        int all = 0, before = 0;
+#pragma unroll 20
+        for (int c = g; c < (int)gridDim.x; c += 4) {
+            const int v = p.counts[c * kDigits + d];
+            all += v;
+            before += c < (int)blockIdx.x ? v : 0;
         }
-        if (lane == 31) warp_sum[warp] = incl;
+        all += __shfl_xor_sync(kFull, all, 8);
+        all += __shfl_xor_sync(kFull, all, 16);
+        before += __shfl_xor_sync(kFull, before, 8);
+        before += __shfl_xor_sync(kFull, before, 16);
+        int incl = all;   // over the warp's digits up to this one
+#pragma unroll
+        for (int s = 1; s < 8; s <<= 1) {
+            const int o = __shfl_up_sync(kFull, incl, s, 8);
+            if ((lane & 7) >= s) incl += o;
+        }
+        if (lane == 7) scan[warp] = incl;
+        __syncthreads();
+        const int warps_before = __reduce_add_sync(kFull, lane < warp ? scan[lane] : 0);
+        if (lane < 8) base[d] = warps_before + incl - all + before;
     }
-    __syncthreads();
-    if (threadIdx.x < kDigits) {
-        for (int w = 0; w < warp; ++w) incl += warp_sum[w];
-        base[d] = incl - mine + before;
-    }
-    const int64_t lo = blockIdx.x * p.part, hi = min(p.n, lo + p.part);
     for (int64_t i0 = lo; i0 < hi; i0 += 1024) {
-        __syncthreads();
-        for (int k = threadIdx.x; k < 32 * kDigits; k += 1024) (&whist[0][0])[k] = 0;
-        __syncthreads();
         const int64_t i = i0 + threadIdx.x;
         const bool in = i < hi;
-        const uint2 e = in ? p.pair(i) : make_uint2(0, 0);
         const int digit = in ? (int)((e.x >> p.shift) & (kDigits - 1)) : 0;
         const unsigned same = same_digit(digit, in);
         const int rank = __popc(same & ((1u << lane) - 1u));
         if (in && rank == 0) whist[warp][digit] = __popc(same);
         __syncthreads();
-        if (threadIdx.x < kDigits) {
-            int run = base[d];
-#pragma unroll 8
-            for (int w = 0; w < 32; ++w) {
-                const int v = whist[w][d];
-                whist[w][d] = run;
-                run += v;
+        {   // four threads a digit, eight warps each
+            const int d = threadIdx.x >> 2, q = threadIdx.x & 3;
+            int v[8], sum = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = whist[q * 8 + k][d];
+                sum += v[k];
             }
-            base[d] = run;
+            int incl = sum;
+            int o = __shfl_up_sync(kFull, incl, 1, 4);
+            if (q >= 1) incl += o;
+            o = __shfl_up_sync(kFull, incl, 2, 4);
+            if (q >= 2) incl += o;
+            int run = base[d] + incl - sum;
+            __syncwarp();
+            if (q == 3) base[d] += incl;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                whist[q * 8 + k][d] = run;
+                run += v[k];
+            }
         }
         __syncthreads();
-        if (in) p.out[whist[warp][digit] + rank] = e;
+        if (in) {
+            const uint32_t to = (uint32_t)(whist[warp][digit] + rank);
+            p.out[to] = e;
+            if (p.next != nullptr) atomicAdd(&p.next[p.per_part.div(to) * kDigits + ((e.x >> (p.shift + 8)) & (kDigits - 1))], 1);
+        }
+        if (i0 + 1024 < hi) {
+            if (i + 1024 < hi) e = p.pair(i + 1024);
+            __syncthreads();
+            for (int k = threadIdx.x; k < 32 * kHistPitch; k += 1024) (&whist[0][0])[k] = 0;
+            __syncthreads();
+        }
     }
 }
 
@@ -425,50 +456,46 @@ struct Sorted {
     __device__ __forceinline__ uint32_t key(int64_t i) const { return pairs[i].x; }
 };
 
-// heads[c] = entries of stretch c that are the first of their id
-__global__ void __launch_bounds__(256) head_count_kernel(Sorted l, int32_t *heads)
+// heads[c] = first entries of their id before stretch c; heads[stretches] and count[0] = all of them.  One cluster, every CTA a contiguous
+// part of the list, read twice: for its own number, and, when the others' are known, for the stretches'.
+__global__ void __launch_bounds__(1024) head_kernel(Sorted l, int32_t *heads, int32_t *count)
 {
-    const int64_t c = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (c >= l.stretches) return;
-    int count = 0;
-    for (int64_t i = c * l.stretch + lane; i < min(l.n, (c + 1) * l.stretch); i += 32) {
-        const uint32_t k = l.key(i);
-        count += k < l.n_nodes && (i == 0 || l.key(i - 1) != k);
-    }
-    count = __reduce_add_sync(kFull, count);
-    if (lane == 0) heads[c] = count;
-}
-
-// heads[c] = first entries before stretch c; heads[stretches] and count[0] = all of them.  One CTA.
-__global__ void __launch_bounds__(1024) head_scan_kernel(int32_t *heads, int64_t stretches, int32_t *count)
-{
-    __shared__ int32_t warp_sum[32];
-    __shared__ int32_t carry;
+    __shared__ int32_t scan[32];
+    __shared__ int32_t total;   // read by the others
+    const uint32_t me = cluster_rank(), size = cluster_size();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) carry = 0;
-    for (int64_t c0 = 0; c0 < stretches; c0 += 1024) {
-        __syncthreads();
-        const int64_t c = c0 + threadIdx.x;
-        const int mine = c < stretches ? heads[c] : 0;
-        int incl = mine;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int v = __shfl_up_sync(kFull, incl, s);
-            if (lane >= s) incl += v;
-        }
-        if (lane == 31) warp_sum[warp] = incl;
-        __syncthreads();
-        const int before = carry + __reduce_add_sync(kFull, lane < warp ? warp_sum[lane] : 0);
-        if (c < stretches) heads[c] = before + incl - mine;
-        __syncthreads();
-        if (threadIdx.x == 1023) carry = before + incl;
-    }
+    const int64_t part = ((l.n + size - 1) / size + l.stretch - 1) / l.stretch * l.stretch;
+    const int64_t lo = min(l.n, me * part), hi = min(l.n, lo + part);
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+    auto is_head = [&](int64_t i) {
+        const uint32_t k = l.key(i);
+        return k < l.n_nodes && (i == 0 || l.key(i - 1) != k);
+    };
+    int mine = 0;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 1024) mine += is_head(i);
+    mine = __reduce_add_sync(kFull, mine);
+    if (lane == 0) scan[warp] = mine;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        heads[stretches] = carry;
+    const int own = __reduce_add_sync(kFull, scan[lane]);
+    if (threadIdx.x == 0) total = own;
+    cluster_sync();
+    int carry = __reduce_add_sync(kFull, (uint32_t)lane < me ? load_cta(in_cta(&total, lane)) : 0);
+    for (int64_t i0 = lo; i0 < hi; i0 += 1024) {
+        const int64_t i = i0 + threadIdx.x;
+        const unsigned first = __ballot_sync(kFull, i < hi && is_head(i));
+        __syncthreads();
+        if (lane == 0) scan[warp] = __popc(first);
+        __syncthreads();
+        const int before = carry + __reduce_add_sync(kFull, lane < warp ? scan[lane] : 0);
+        if (lane == 0 && i < hi && i % l.stretch == 0) heads[i / l.stretch] = before;   // stretches are whole warps
+        carry += __reduce_add_sync(kFull, scan[lane]);
+    }
+    if (threadIdx.x == 0 && me == size - 1) {
+        heads[l.stretches] = carry;
         count[0] = carry;
     }
+    cluster_sync();  // no CTA's memory goes while another one may read it
 }
 
 struct GradOut {
@@ -539,6 +566,8 @@ grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradO
     const int64_t c = (int64_t)blockIdx.x * (kSumThreads >> log_group) + group;
     if (c >= l.stretches || col >= o.dim) return;
     const int64_t lo = c * l.stretch, hi = min(l.n, lo + l.stretch);
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     uint32_t key[kAhead];
     Vec<T, VE> next[kAhead];
     auto fetch = [&](int64_t i0, uint32_t *k, Vec<T, VE> *v) {
@@ -616,6 +645,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(Sorted l, GradOu
     const int col = ((int)blockIdx.y * kSumThreads + in_group) * VE;
     const int64_t c = (int64_t)blockIdx.x * groups + (threadIdx.x >> log_group), lo = c * l.stretch, hi = lo + l.stretch;
     if (threadIdx.x == 0) longs = 0;
+    cudaGridDependencySynchronize();
     __syncthreads();
     if (c < l.stretches && hi < l.n) {
         const uint32_t k = l.key(hi - 1), behind = l.key(hi), before = lo > 0 ? l.key(lo - 1) : 0xFFFFFFFFu;
@@ -859,7 +889,7 @@ struct GradScratch {
         };
         const int64_t stretches = (n + stretch_of(n) - 1) / stretch_of(n);
         for (int k = 0; k < 2; ++k) pairs[k] = (uint2 *)take(8 * n);
-        counts = (int32_t *)take((int64_t)kSms * kDigits * 4);
+        counts = (int32_t *)take((int64_t)kPassMax * kSms * kDigits * 4);
         heads = (int32_t *)take(n <= kDirectMax ? kDirectMax / 8 : 4 * (stretches + 1));
         head_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
         tail_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
@@ -895,6 +925,33 @@ static int widest_cluster()
     return found[dev];
 }
 
+// A launch in clusters of `cluster` CTAs (0: none), `after_own`: as a dependent of this file's launch before it, which it may overlap
+// up to its cudaGridDependencySynchronize.
+template <typename... A, typename... B>
+static cudaError_t launch(cudaStream_t s, void (*kernel)(A...), unsigned grid_x, unsigned grid_y, unsigned threads, int64_t smem, unsigned cluster,
+                          bool after_own, B... args)
+{
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid_x, grid_y);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    if (cluster > 0) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (after_own) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, A(args)...);
+}
+
 static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch &w, int32_t *count, const ZeroFill &fill, Sorted *l)
 {
     l->n = n;
@@ -904,7 +961,7 @@ static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch
     int bits = 0;
     while ((ids.n_nodes >> bits) != 0) ++bits;  // n_nodes itself is a key
     const int widest = widest_cluster();
-    if (n <= (int64_t)widest * kClusterPart) {
+    if (n <= kClusterList && n <= (int64_t)widest * kClusterPart) {
         int ctas = 1;
         while (ctas < widest && (int64_t)ctas * kClusterThreads < n) ctas *= 2;
         const int64_t part = ((n + ctas - 1) / ctas + kClusterThreads - 1) / kClusterThreads * kClusterThreads;
@@ -914,18 +971,7 @@ static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch
         int64_t fillers = fill.p != nullptr ? (fill.rows * fill.width + (128 << 10) - 1) / (128 << 10) : 0;
         if (fillers > 112) fillers = 112;
         fillers = (fillers + ctas - 1) / ctas * ctas;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)ctas;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(ctas + fillers));
-        cfg.blockDim = dim3(kClusterThreads);
-        cfg.dynamicSmemBytes = (size_t)cluster_sort_smem(part);
-        cfg.stream = s;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        LG_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel, p));
+        LG_CUDA(launch(s, cluster_sort_kernel, (unsigned)(ctas + fillers), 1, kClusterThreads, cluster_sort_smem(part), (unsigned)ctas, false, p));
         l->pairs = w.pairs[0];
         return LEGION_OK;
     }
@@ -933,38 +979,34 @@ static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch
         if (fill.pitch == fill.width) LG_CUDA(cudaMemsetAsync(fill.p, 0, (size_t)(fill.rows * fill.width), s));
         else LG_CUDA(cudaMemset2DAsync(fill.p, (size_t)fill.pitch, 0, (size_t)fill.width, (size_t)fill.rows, s));
     }
-    SortPass p;
-    p.ids = ids;
-    p.counts = w.counts;
-    p.n = n;
-    const int64_t ctas = kSms;
-    p.part = (n + ctas - 1) / ctas;
-    int to = 0;
-    for (p.shift = 0; p.shift < bits; p.shift += 8, to ^= 1) {
-        p.in = p.shift == 0 ? nullptr : w.pairs[to ^ 1];
-        p.out = w.pairs[to];
-        sort_count_kernel<<<(unsigned)ctas, 1024, 0, s>>>(p);
-        sort_scatter_kernel<<<(unsigned)ctas, 1024, 0, s>>>(p);
+    const int part = (int)((n + kSms - 1) / kSms);
+    SortPass p{ ids, nullptr, nullptr, w.counts, nullptr, n, part, FastDiv((uint32_t)part), 0 };
+    const int passes = (bits + 7) / 8;
+    LG_CUDA(launch(s, sort_count_kernel, kSms, 1, 1024, 0, 0, false, p, passes));
+    for (int q = 0; q < passes; ++q) {
+        p.in = q == 0 ? nullptr : w.pairs[(q & 1) ^ 1];
+        p.out = w.pairs[q & 1];
+        p.counts = w.counts + q * kSms * kDigits;
+        p.next = q + 1 < passes ? w.counts + (q + 1) * kSms * kDigits : nullptr;
+        p.shift = q * 8;
+        LG_CUDA(launch(s, sort_scatter_kernel, kSms, 1, 1024, 0, 0, true, p));
     }
-    l->pairs = w.pairs[to ^ 1];
-    if (count != nullptr) {
-        head_count_kernel<<<(unsigned)((l->stretches + 7) / 8), 256, 0, s>>>(*l, w.heads);
-        head_scan_kernel<<<1, 1024, 0, s>>>(w.heads, l->stretches, count);
-    }
-    LG_LAUNCH_CHECK();
+    l->pairs = w.pairs[(passes & 1) ^ 1];
+    if (count != nullptr) LG_CUDA(launch(s, head_kernel, 8, 1, 1024, 0, 8, true, *l, w.heads, count));
     return LEGION_OK;
 }
 
 template <typename T, int VE>
-static void launch_sum(cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
+static int launch_sum(cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
 {
     const int vecs = o.dim / VE;
     int log_group = 0;
     while ((1 << log_group) < kSumThreads && (1 << log_group) < vecs) ++log_group;
     const int64_t per = kSumThreads >> log_group;
     const dim3 grid((unsigned)((l.stretches + per - 1) / per), (unsigned)((vecs + kSumThreads - 1) / kSumThreads));
-    grad_sum_kernel<T, VE><<<grid, kSumThreads, 0, s>>>(l, (const T *)grad, stride, o, log_group);
-    if (l.stretches > 1) grad_join_kernel<VE><<<grid, kSumThreads, 0, s>>>(l, o, log_group);
+    LG_CUDA(launch(s, grad_sum_kernel<T, VE>, grid.x, grid.y, kSumThreads, 0, 0, true, l, (const T *)grad, stride, o, log_group));
+    if (l.stretches > 1) LG_CUDA(launch(s, grad_join_kernel<VE>, grid.x, grid.y, kSumThreads, 0, 0, true, l, o, log_group));
+    return LEGION_OK;
 }
 
 template <typename T, int VE>
@@ -991,14 +1033,14 @@ static void launch_direct_ve(int ve, cudaStream_t s, const Direct &d, const void
 }
 
 template <typename T>
-static void launch_sum_ve(int ve, cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
+static int launch_sum_ve(int ve, cudaStream_t s, const Sorted &l, const void *grad, int64_t stride, const GradOut &o)
 {
     switch (ve) {
     case 8:
-        if constexpr (sizeof(T) == 2) { launch_sum<T, 8>(s, l, grad, stride, o); break; }
-    case 4: launch_sum<T, 4>(s, l, grad, stride, o); break;
-    case 2: launch_sum<T, 2>(s, l, grad, stride, o); break;
-    default: launch_sum<T, 1>(s, l, grad, stride, o); break;
+        if constexpr (sizeof(T) == 2) return launch_sum<T, 8>(s, l, grad, stride, o);
+    case 4: return launch_sum<T, 4>(s, l, grad, stride, o);
+    case 2: return launch_sum<T, 2>(s, l, grad, stride, o);
+    default: return launch_sum<T, 1>(s, l, grad, stride, o);
     }
 }
 
@@ -1026,11 +1068,9 @@ static int run_grad(cudaStream_t s, const Ids &ids, int64_t n, const void *grad,
     o.head_part = w.head_part;
     o.tail_part = w.tail_part;
     o.heads = count != nullptr ? w.heads : nullptr;
-    if (grad_dtype == LEGION_F32) launch_sum_ve<float>(ve, s, l, grad, grad_stride, o);
-    else if (grad_dtype == LEGION_F16) launch_sum_ve<__half>(ve, s, l, grad, grad_stride, o);
-    else launch_sum_ve<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
-    LG_LAUNCH_CHECK();
-    return LEGION_OK;
+    if (grad_dtype == LEGION_F32) return launch_sum_ve<float>(ve, s, l, grad, grad_stride, o);
+    if (grad_dtype == LEGION_F16) return launch_sum_ve<__half>(ve, s, l, grad, grad_stride, o);
+    return launch_sum_ve<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
 }
 
 }  // namespace legion
