@@ -106,11 +106,11 @@ constexpr int kDigits = 256;
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterItems = 11;                            // entries that a thread has at most
 constexpr int kClusterPart = kClusterItems * kClusterThreads; // entries that a CTA has at most
-constexpr int64_t kClusterList = 32768;                      // longest list that a cluster sorts
+constexpr int64_t kClusterList = 20480;   // longest list that a cluster sorts (16384 ids: 30 us a call, 31 by the passes below; 32768: 33 and 32)
 constexpr int kHistPitch = kDigits + 1;                      // the 32 counts of a digit lie in 32 banks
 
-// The rows of the gradient that no id names are zeros: the CTAs of the sorting launch that have nothing to sort write them (all
-// rows; those that are named are written again by the sums).
+// The rows of the gradient that no id names are zeros: a launch of its own writes them, all rows (those that are named are written again by
+// the sums), and the sort inside a cluster runs beside it.
 struct ZeroFill {
     uint8_t *p;            // nullptr: nothing to fill
     int64_t rows, width, pitch;  // bytes of a row, bytes from row to row
@@ -129,7 +129,6 @@ __device__ __forceinline__ void zero_run(uint8_t *p, int64_t bytes, int64_t at, 
 }
 __device__ __forceinline__ void zero_fill(const ZeroFill &z, int64_t at, int64_t threads)
 {
-    if (z.p == nullptr) return;
     if (z.pitch == z.width) {
         zero_run(z.p, z.rows * z.width, at, threads);
     } else {
@@ -149,6 +148,13 @@ __device__ __forceinline__ unsigned same_digit(int digit, bool in)
     return same;
 }
 
+// Bound by HBM's writes: 7 TB/s with four CTAs on every SM (112 CTAs of the sort's own launch wrote 4.8).
+__global__ void __launch_bounds__(256) zero_fill_kernel(ZeroFill z)
+{
+    cudaTriggerProgrammaticLaunchCompletion();
+    zero_fill(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
 struct ClusterSort {
     Ids ids;
     int32_t n, part;      // entries; entries per CTA, a multiple of kClusterThreads
@@ -158,7 +164,6 @@ struct ClusterSort {
     int32_t *heads;       // rows that occur: first entries before every stretch (GradOut), or nullptr
     int32_t *count;
     int32_t stretch;      // a multiple of 32
-    ZeroFill fill;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -191,15 +196,11 @@ __host__ __device__ constexpr int64_t cluster_sort_smem(int64_t part) { return p
 // between the passes.  A warp has 32 * items entries one behind the other and ranks them in list order; counts of
 // the CTAs' digits are read out of each other's shared memory, entries are written straight to the CTA that has their place.
 // What bounds it is latency (two cluster barriers a pass), so the entries are spread over up to 16 CTAs even when one could hold them.
-// Clusters behind the first one write the zero rows of the gradient meanwhile.
+// It does not wait for the launch before it, the zero rows, until its own work is done: what follows it may write over them.
 __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(ClusterSort p)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t size = cluster_size();
-    if (blockIdx.x >= size) {
-        zero_fill(p.fill, (int64_t)(blockIdx.x - size) * kClusterThreads + threadIdx.x, (int64_t)(gridDim.x - size) * kClusterThreads);
-        return;
-    }
     cudaTriggerProgrammaticLaunchCompletion();
     const uint32_t me = cluster_rank();
     uint2 *buf[2] = { reinterpret_cast<uint2 *>(smem), reinterpret_cast<uint2 *>(smem) + p.part };
@@ -324,44 +325,59 @@ __global__ void __launch_bounds__(kClusterThreads, 1) cluster_sort_kernel(Cluste
         const int i = threadIdx.x * 32;
         if (threadIdx.x < pieces && i < mine && (first + i) % p.stretch == 0) p.heads[(first + i) / p.stretch] = before + excl;
         if (threadIdx.x == 0 && me == size - 1) {
-            p.heads[(p.n + p.stretch - 1) / p.stretch] = before + of_cta;
             p.count[0] = before + of_cta;
         }
     }
+    cudaGridDependencySynchronize();
     cluster_sync();  // no CTA's memory goes while another one may read it
 }
 
-// Longer lists: the same passes over global memory, every CTA one contiguous part of the list.  A pass is one launch: it reads the counts
-// of all parts' digits, and counts the next pass's digits of the parts that its entries go to (whole numbers: the order of the
-// atomics changes nothing).  What bounds a pass is the chain of latencies in it; the launches are dependents that start while the one
-// before ends.
+// Longer lists: the same passes over global memory, every CTA one contiguous part of the list.  A pass counts the parts' digits
+// and then moves the entries.  Counts are kept for every part and for groups of kGroup parts (whole numbers: the order of the atomics
+// changes nothing): a CTA reads those of its group and of the other groups, 25 rows in place of 148 (every CTA reading all
+// counts took 14000 of a move's 20000 clocks; counting the next pass's digits by atomics while entries move took 6 us, a launch for
+// it 3.5).  What bounds a pass is the chain of latencies in it; the launches are dependents that start while the one before ends.
 constexpr int kPassMax = 4;
+constexpr int kGroup = 12, kGroups = (kSms + kGroup - 1) / kGroup;
+constexpr int kCountRows = kSms + kGroups;   // the parts', then the groups'
+__device__ __forceinline__ void count_digit(int32_t *counts, uint32_t part, int digit, int v)
+{
+    atomicAdd(&counts[part * kDigits + digit], v);
+    atomicAdd(&counts[(kSms + part / kGroup) * kDigits + digit], v);
+}
 struct SortPass {
     Ids ids;                  // first pass: the ids themselves
     const uint2 *in;          // later ones: the pairs
     uint2 *out;
-    int32_t *counts;          // [CTA][digit] of this pass
-    int32_t *next;            // of the next one, or nullptr
+    int32_t *counts;          // [kCountRows][digit] of this pass
     int64_t n;
     int32_t part;             // entries per CTA
-    FastDiv per_part;
     int32_t shift;
     __device__ __forceinline__ uint2 pair(int64_t i) const { return in != nullptr ? in[i] : make_uint2(ids.key(i), (uint32_t)i); }
 };
 
-// The first pass's counts; the others' are zeroed.
-__global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p, int passes)
+// Counts of all passes and the ticket behind them: zeros.
+__global__ void __launch_bounds__(1024) sort_zero_kernel(int32_t *counts, int words)
+{
+    cudaTriggerProgrammaticLaunchCompletion();
+    for (int i = blockIdx.x * 1024 + threadIdx.x; i < words; i += gridDim.x * 1024) counts[i] = 0;
+}
+
+__global__ void __launch_bounds__(1024) sort_count_kernel(SortPass p)
 {
     __shared__ int32_t hist[kDigits];
     if (threadIdx.x < kDigits) hist[threadIdx.x] = 0;
-    for (int q = 1; q < passes; ++q)
-        for (int i = threadIdx.x; i < kDigits; i += blockDim.x) p.counts[(q * kSms + blockIdx.x) * kDigits + i] = 0;
     cudaTriggerProgrammaticLaunchCompletion();
+    if (p.in != nullptr) cudaGridDependencySynchronize();   // the ids are there already
     __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * p.part, hi = min(p.n, lo + p.part);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&hist[p.ids.key(i) & (kDigits - 1)], 1);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+        const uint32_t key = p.in != nullptr ? p.in[i].x : p.ids.key(i);
+        atomicAdd(&hist[(key >> p.shift) & (kDigits - 1)], 1);
+    }
     __syncthreads();
-    if (threadIdx.x < kDigits) p.counts[blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
+    if (p.in == nullptr) cudaGridDependencySynchronize();
+    if (threadIdx.x < kDigits && hist[threadIdx.x] != 0) count_digit(p.counts, blockIdx.x, threadIdx.x, hist[threadIdx.x]);
 }
 
 __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
@@ -376,14 +392,20 @@ __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
     const int64_t lo = (int64_t)blockIdx.x * p.part, hi = min(p.n, lo + p.part);
     uint2 e = lo + threadIdx.x < hi ? p.pair(lo + threadIdx.x) : make_uint2(0, 0);
     {   // entries of smaller digits, and of the same digit in the parts before this one; warp w has digits 8 w to 8 w + 7, a quarter
-        // of the parts per eight lanes
-        const int d = warp * 8 + (lane & 7), g = lane >> 3;
+        // of the counts per eight lanes
+        const int d = warp * 8 + (lane & 7), q = lane >> 3, group = blockIdx.x / kGroup, in_group = blockIdx.x - group * kGroup;
         int all = 0, before = 0;
-#pragma unroll 20
-        for (int c = g; c < (int)gridDim.x; c += 4) {
-            const int v = p.counts[c * kDigits + d];
+#pragma unroll
+        for (int j = 0; j < (kGroups + 3) / 4; ++j) {
+            const int c = 4 * j + q;
+            const int v = c < kGroups ? p.counts[(kSms + c) * kDigits + d] : 0;
             all += v;
-            before += c < (int)blockIdx.x ? v : 0;
+            before += c < group ? v : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kGroup / 4; ++j) {
+            const int c = 4 * j + q;
+            if (c < in_group) before += p.counts[(group * kGroup + c) * kDigits + d];
         }
         all += __shfl_xor_sync(kFull, all, 8);
         all += __shfl_xor_sync(kFull, all, 16);
@@ -431,11 +453,7 @@ __global__ void __launch_bounds__(1024) sort_scatter_kernel(SortPass p)
             }
         }
         __syncthreads();
-        if (in) {
-            const uint32_t to = (uint32_t)(whist[warp][digit] + rank);
-            p.out[to] = e;
-            if (p.next != nullptr) atomicAdd(&p.next[p.per_part.div(to) * kDigits + ((e.x >> (p.shift + 8)) & (kDigits - 1))], 1);
-        }
+        if (in) p.out[whist[warp][digit] + rank] = e;
         if (i0 + 1024 < hi) {
             if (i + 1024 < hi) e = p.pair(i + 1024);
             __syncthreads();
@@ -456,46 +474,65 @@ struct Sorted {
     __device__ __forceinline__ uint32_t key(int64_t i) const { return pairs[i].x; }
 };
 
-// heads[c] = first entries of their id before stretch c; heads[stretches] and count[0] = all of them.  One cluster, every CTA a contiguous
-// part of the list, read twice: for its own number, and, when the others' are known, for the stretches'.
-__global__ void __launch_bounds__(1024) head_kernel(Sorted l, int32_t *heads, int32_t *count)
+// First entries of their id before every stretch: `local` counts from the start of the stretch's part on, `base` is the part's (nullptr:
+// local counts from the list's start); count[0] = all of them.
+struct Heads {
+    int32_t *local, *base, *count;
+    FastDiv per_part;   // stretches
+    int64_t stretches;
+    __device__ __forceinline__ int32_t before(int64_t stretch) const
+    {
+        if (stretch >= stretches) return count[0];
+        return local[stretch] + (base != nullptr ? base[per_part.div((uint32_t)stretch)] : 0);
+    }
+};
+
+// Every CTA has a part of the list; the last one to end turns the parts' numbers into sums.
+__global__ void __launch_bounds__(1024) head_kernel(Sorted l, Heads h, int32_t *ticket)
 {
     __shared__ int32_t scan[32];
-    __shared__ int32_t total;   // read by the others
-    const uint32_t me = cluster_rank(), size = cluster_size();
+    __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t part = ((l.n + size - 1) / size + l.stretch - 1) / l.stretch * l.stretch;
-    const int64_t lo = min(l.n, me * part), hi = min(l.n, lo + part);
+    const int64_t part = (int64_t)h.per_part.d * l.stretch, lo = min(l.n, blockIdx.x * part), hi = min(l.n, lo + part);
     cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
-    auto is_head = [&](int64_t i) {
-        const uint32_t k = l.key(i);
-        return k < l.n_nodes && (i == 0 || l.key(i - 1) != k);
-    };
-    int mine = 0;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 1024) mine += is_head(i);
-    mine = __reduce_add_sync(kFull, mine);
-    if (lane == 0) scan[warp] = mine;
-    __syncthreads();
-    const int own = __reduce_add_sync(kFull, scan[lane]);
-    if (threadIdx.x == 0) total = own;
-    cluster_sync();
-    int carry = __reduce_add_sync(kFull, (uint32_t)lane < me ? load_cta(in_cta(&total, lane)) : 0);
+    int carry = 0;
     for (int64_t i0 = lo; i0 < hi; i0 += 1024) {
         const int64_t i = i0 + threadIdx.x;
-        const unsigned first = __ballot_sync(kFull, i < hi && is_head(i));
+        bool head = false;
+        if (i < hi) {
+            const uint32_t k = l.key(i);
+            head = k < l.n_nodes && (i == 0 || l.key(i - 1) != k);
+        }
+        const unsigned first = __ballot_sync(kFull, head);
         __syncthreads();
         if (lane == 0) scan[warp] = __popc(first);
         __syncthreads();
         const int before = carry + __reduce_add_sync(kFull, lane < warp ? scan[lane] : 0);
-        if (lane == 0 && i < hi && i % l.stretch == 0) heads[i / l.stretch] = before;   // stretches are whole warps
+        if (lane == 0 && i < hi && i % l.stretch == 0) h.local[i / l.stretch] = before;   // stretches are whole warps
         carry += __reduce_add_sync(kFull, scan[lane]);
     }
-    if (threadIdx.x == 0 && me == size - 1) {
-        heads[l.stretches] = carry;
-        count[0] = carry;
+    if (threadIdx.x == 0) {
+        h.base[blockIdx.x] = carry;
+        __threadfence();
+        last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
     }
-    cluster_sync();  // no CTA's memory goes while another one may read it
+    __syncthreads();
+    if (!last || warp != 0) return;
+    __threadfence();
+    int sum = 0;
+    for (int c0 = 0; c0 < (int)gridDim.x; c0 += 32) {
+        const int mine = c0 + lane < (int)gridDim.x ? __ldcg(&h.base[c0 + lane]) : 0;
+        int incl = mine;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int o = __shfl_up_sync(kFull, incl, s);
+            if (lane >= s) incl += o;
+        }
+        if (c0 + lane < (int)gridDim.x) h.base[c0 + lane] = sum + incl - mine;
+        sum += __shfl_sync(kFull, incl, 31);
+    }
+    if (lane == 0) h.count[0] = sum;
 }
 
 struct GradOut {
@@ -503,7 +540,7 @@ struct GradOut {
     int64_t stride;
     int32_t dtype;
     int32_t accumulate;
-    const int32_t *heads; // rows that occur: first entries before every stretch; whole table: nullptr
+    Heads heads;          // rows that occur: first entries before every stretch; whole table: local is nullptr
     void *unique;         // rows that occur: their ids
     int32_t wide;
     float scale;
@@ -581,7 +618,7 @@ grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradO
         }
     };
     const uint32_t prev = lo > 0 ? l.key(lo - 1) : 0xFFFFFFFFu, behind = hi < l.n ? l.key(hi) : 0xFFFFFFFFu;
-    const int32_t heads = o.heads != nullptr ? o.heads[c] : 0;
+    const int32_t heads = o.heads.local != nullptr ? o.heads.before(c) : 0;
     fetch(lo, key, next);
     uint32_t cur = key[0];
     if (cur >= l.n_nodes) return;
@@ -592,7 +629,7 @@ grad_sum_kernel(Sorted l, const T *__restrict__ grad, int64_t grad_stride, GradO
     for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
     auto flush = [&]() {
         if (open) store_part<VE>(o.head_part + c * o.dim + col, acc);
-        else o.put<VE>(o.heads != nullptr ? seg : (int64_t)cur, col, acc);
+        else o.put<VE>(o.heads.local != nullptr ? seg : (int64_t)cur, col, acc);
     };
     auto name = [&]() {
         if (o.unique != nullptr && col == 0 && !open) {
@@ -658,7 +695,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(Sorted l, GradOu
             }
             for (; step >= 1; step /= 2)
                 if (last + step < l.stretches && l.key((last + step) * l.stretch) == k) last += step;
-            const int64_t row = o.heads != nullptr ? o.heads[c + 1] - 1 : (int64_t)k;
+            const int64_t row = o.heads.local != nullptr ? o.heads.before(c + 1) - 1 : (int64_t)k;
             if (last - c >= kLong) {
                 if (in_group == 0) {
                     const int at = atomicAdd(&longs, 1);   // in which order they are taken changes nothing
@@ -682,7 +719,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(Sorted l, GradOu
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     for (int q = 0; q < longs; ++q) {
         const int64_t first = long_first[q], last = long_last[q];
-        const int64_t row = o.heads != nullptr ? o.heads[first + 1] - 1 : (int64_t)l.key((first + 1) * l.stretch);
+        const int64_t row = o.heads.local != nullptr ? o.heads.before(first + 1) - 1 : (int64_t)l.key((first + 1) * l.stretch);
         const int end = min(o.dim, ((int)blockIdx.y + 1) * kSumThreads * VE);
         for (int col0 = (int)blockIdx.y * kSumThreads * VE; col0 < end; col0 += 32 * VE) {
             const int at = col0 + x * VE;
@@ -889,7 +926,7 @@ struct GradScratch {
         };
         const int64_t stretches = (n + stretch_of(n) - 1) / stretch_of(n);
         for (int k = 0; k < 2; ++k) pairs[k] = (uint2 *)take(8 * n);
-        counts = (int32_t *)take((int64_t)kPassMax * kSms * kDigits * 4);
+        counts = (int32_t *)take(((int64_t)kPassMax * kCountRows * kDigits + 1 + kSms) * 4);   // and a ticket, and the parts' first entries
         heads = (int32_t *)take(n <= kDirectMax ? kDirectMax / 8 : 4 * (stretches + 1));
         head_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
         tail_part = (float *)take(stretches > 1 ? 4 * stretches * dim : 0);
@@ -952,7 +989,7 @@ static cudaError_t launch(cudaStream_t s, void (*kernel)(A...), unsigned grid_x,
     return cudaLaunchKernelEx(&cfg, kernel, A(args)...);
 }
 
-static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch &w, int32_t *count, const ZeroFill &fill, Sorted *l)
+static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch &w, int32_t *count, const ZeroFill &fill, Sorted *l, Heads *heads)
 {
     l->n = n;
     l->n_nodes = (uint32_t)ids.n_nodes;
@@ -965,14 +1002,14 @@ static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch
         int ctas = 1;
         while (ctas < widest && (int64_t)ctas * kClusterThreads < n) ctas *= 2;
         const int64_t part = ((n + ctas - 1) / ctas + kClusterThreads - 1) / kClusterThreads * kClusterThreads;
-        ClusterSort p{ ids, (int32_t)n, (int32_t)part, FastDiv((uint32_t)part), bits, w.pairs[0], count != nullptr ? w.heads : nullptr, count, l->stretch, fill };
-        // a CTA that fills has 128 KB or more to write; no more of them than surely run at one time beside the sort (clusters of 16 fit
-        // once into each of eight groups of SMs)
-        int64_t fillers = fill.p != nullptr ? (fill.rows * fill.width + (128 << 10) - 1) / (128 << 10) : 0;
-        if (fillers > 112) fillers = 112;
-        fillers = (fillers + ctas - 1) / ctas * ctas;
-        LG_CUDA(launch(s, cluster_sort_kernel, (unsigned)(ctas + fillers), 1, kClusterThreads, cluster_sort_smem(part), (unsigned)ctas, false, p));
+        ClusterSort p{ ids, (int32_t)n, (int32_t)part, FastDiv((uint32_t)part), bits, w.pairs[0], count != nullptr ? w.heads : nullptr, count, l->stretch };
+        if (fill.p != nullptr) {
+            const int64_t need = (fill.rows * fill.width + 16383) / 16384;   // 16 KB a CTA or more
+            LG_CUDA(launch(s, zero_fill_kernel, (unsigned)(need < 4 * kSms ? need : 4 * kSms), 1, 256, 0, 0, false, fill));
+        }
+        LG_CUDA(launch(s, cluster_sort_kernel, (unsigned)ctas, 1, kClusterThreads, cluster_sort_smem(part), (unsigned)ctas, fill.p != nullptr, p));
         l->pairs = w.pairs[0];
+        if (count != nullptr) *heads = Heads{ w.heads, nullptr, count, FastDiv(1), l->stretches };
         return LEGION_OK;
     }
     if (fill.p != nullptr) {
@@ -980,19 +1017,24 @@ static int sort_ids(cudaStream_t s, const Ids &ids, int64_t n, const GradScratch
         else LG_CUDA(cudaMemset2DAsync(fill.p, (size_t)fill.pitch, 0, (size_t)fill.width, (size_t)fill.rows, s));
     }
     const int part = (int)((n + kSms - 1) / kSms);
-    SortPass p{ ids, nullptr, nullptr, w.counts, nullptr, n, part, FastDiv((uint32_t)part), 0 };
-    const int passes = (bits + 7) / 8;
-    LG_CUDA(launch(s, sort_count_kernel, kSms, 1, 1024, 0, 0, false, p, passes));
+    SortPass p{ ids, nullptr, nullptr, w.counts, n, part, 0 };
+    const int passes = (bits + 7) / 8, words = passes * kCountRows * kDigits;
+    int32_t *ticket = w.counts + words;
+    LG_CUDA(launch(s, sort_zero_kernel, 64, 1, 1024, 0, 0, false, w.counts, words + 1));
     for (int q = 0; q < passes; ++q) {
         p.in = q == 0 ? nullptr : w.pairs[(q & 1) ^ 1];
         p.out = w.pairs[q & 1];
-        p.counts = w.counts + q * kSms * kDigits;
-        p.next = q + 1 < passes ? w.counts + (q + 1) * kSms * kDigits : nullptr;
+        p.counts = w.counts + q * kCountRows * kDigits;
         p.shift = q * 8;
+        LG_CUDA(launch(s, sort_count_kernel, kSms, 1, 1024, 0, 0, true, p));
         LG_CUDA(launch(s, sort_scatter_kernel, kSms, 1, 1024, 0, 0, true, p));
     }
     l->pairs = w.pairs[(passes & 1) ^ 1];
-    if (count != nullptr) LG_CUDA(launch(s, head_kernel, 8, 1, 1024, 0, 8, true, *l, w.heads, count));
+    if (count != nullptr) {
+        const uint32_t per_part = (uint32_t)((l->stretches + kSms - 1) / kSms);
+        *heads = Heads{ w.heads, ticket + 1, count, FastDiv(per_part), l->stretches };
+        LG_CUDA(launch(s, head_kernel, (unsigned)((l->stretches + per_part - 1) / per_part), 1, 1024, 0, 0, true, *l, *heads, ticket));
+    }
     return LEGION_OK;
 }
 
@@ -1063,11 +1105,12 @@ static int run_grad(cudaStream_t s, const Ids &ids, int64_t n, const void *grad,
         return LEGION_OK;
     }
     Sorted l;
-    int rc = sort_ids(s, ids, n, w, count, fill, &l);
+    Heads heads{ nullptr, nullptr, nullptr, FastDiv(1), 0 };
+    int rc = sort_ids(s, ids, n, w, count, fill, &l, &heads);
     if (rc != LEGION_OK) return rc;
     o.head_part = w.head_part;
     o.tail_part = w.tail_part;
-    o.heads = count != nullptr ? w.heads : nullptr;
+    o.heads = heads;
     if (grad_dtype == LEGION_F32) return launch_sum_ve<float>(ve, s, l, grad, grad_stride, o);
     if (grad_dtype == LEGION_F16) return launch_sum_ve<__half>(ve, s, l, grad, grad_stride, o);
     return launch_sum_ve<__nv_bfloat16>(ve, s, l, grad, grad_stride, o);
@@ -1154,7 +1197,7 @@ extern "C" int legion_embedding_grad(int32_t dev_id, const void *ids, int32_t id
         return LEGION_OK;
     }
     const ZeroFill fill{ accumulate ? nullptr : (uint8_t *)grad_table, n_nodes, width, pitch };
-    GradOut o{};
+    GradOut o{ nullptr, 0, 0, 0, Heads{ nullptr, nullptr, nullptr, FastDiv(1), 0 }, nullptr, 0, 0.0f, 0, nullptr, nullptr };
     o.rows = grad_table;
     o.stride = table_stride;
     o.dtype = table_dtype;
@@ -1184,7 +1227,7 @@ extern "C" int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32
         LG_CUDA(cudaMemsetAsync(count, 0, 4, s));
         return LEGION_OK;
     }
-    GradOut o{};
+    GradOut o{ nullptr, 0, 0, 0, Heads{ nullptr, nullptr, nullptr, FastDiv(1), 0 }, nullptr, 0, 0.0f, 0, nullptr, nullptr };
     o.rows = grad_rows;
     o.stride = rows_stride;
     o.dtype = LEGION_F32;
