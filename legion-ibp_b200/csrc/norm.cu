@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
             }
         }
     };
-    constexpr bool kAhead = U * VE <= 16;   // wider threads have no registers for it
+    constexpr bool kAhead = U * VE <= 16 || GROUP == 32;   // wider threads of a CTA have no registers for it
     const int64_t step = (int64_t)gridDim.x * per_cta;
     if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
     float w[U][VE];
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
             }
         }
     };
-    constexpr bool kAhead = U * VE <= 16;   // wider threads have no registers for it
+    constexpr bool kAhead = U * VE <= 16 || GROUP == 32;   // wider threads of a CTA have no registers for it
     const int64_t step = (int64_t)gridDim.x * per_cta;
     if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
     float w[U][VE], dw[U][VE];
@@ -333,15 +333,16 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float *__r
 
 constexpr int kGradCtas = 4 * kSms;  // most CTAs of the gradient: their shares of the weight's gradient lie in scratch
 
-// How a row of `vecs` vectors is held: lanes of a warp as long as four vectors a lane hold it, a CTA behind that.
+// How a row of `vecs` vectors is held: by 8 lanes, by a warp (up to 32 elements a lane where there are many rows: nobody waits at a
+// barrier then), or by a CTA.
 struct RowShape {
     int group, u, threads, per_cta;
 };
-static RowShape row_shape(int vecs, int64_t n)
+static RowShape row_shape(int vecs, int ve, int64_t n)
 {
     if (vecs <= 8) return { 8, 1, 128, 16 };
-    if (vecs <= 32) return { 32, 1, 128, 4 };
-    if (vecs <= 64) return { 32, 2, 128, 4 };
+    for (int w = 1; w <= 16 && w * ve <= 32 && (w == 1 || n >= 8 * kSms); w *= 2)
+        if (vecs <= 32 * w) return { 32, w, 128, 4 };
     int u = 1;  // few rows: as many threads as there are vectors; many: CTAs of about 256 threads, so that several are on an SM
     if (n >= 2 * kSms)
         while (u < 4 && (vecs + u - 1) / u > 256) u *= 2;
@@ -362,7 +363,7 @@ static unsigned resident(int64_t need, const void *kernel, int threads, int per_
 template <typename T, int VE, int CODEC>
 static int launch_norm(cudaStream_t s, const NormParams &p)
 {
-    const RowShape r = row_shape(p.dim / VE, p.n);
+    const RowShape r = row_shape(p.dim / VE, VE, p.n);
     const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
 #define LG_NORM(U, GROUP, MAXT)                                                                                                     \
     norm_kernel<T, VE, U, GROUP, CODEC, MAXT><<<resident(need, (const void *)norm_kernel<T, VE, U, GROUP, CODEC, MAXT>, r.threads, 16), \
@@ -370,7 +371,13 @@ static int launch_norm(cudaStream_t s, const NormParams &p)
 // a CTA of at most 256 threads may have twice the registers of a thread of one of 512
 #define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, 512); } while (0)
     if (r.group == 8) LG_NORM(1, 8, 128);
-    else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
+    else if (r.group == 32) {
+        if (r.u == 1) LG_NORM(1, 32, 128);
+        else if (r.u == 2) LG_NORM(2, 32, 128);
+        else if (r.u == 4) LG_NORM(4, 32, 128);
+        else if (r.u == 8) { if constexpr (VE <= 4) LG_NORM(8, 32, 128); }
+        else { if constexpr (VE <= 2) LG_NORM(16, 32, 128); }
+    }
     else if (r.u == 1) LG_NORM_CTA(1);
     else if (r.u == 2) LG_NORM_CTA(2);
     else if (r.u == 4) LG_NORM_CTA(4);
@@ -406,7 +413,7 @@ static int launch_norm_codec(cudaStream_t s, const NormParams &p, int codec, int
 template <typename T, int VE>
 static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
 {
-    const RowShape r = row_shape(p.dim / VE, p.n);
+    const RowShape r = row_shape(p.dim / VE, VE, p.n);
     const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
 #define LG_NORM(U, GROUP, MAXT)                                                                                                    \
     norm_grad_kernel<T, VE, U, GROUP, MAXT><<<*parts = resident(need, (const void *)norm_grad_kernel<T, VE, U, GROUP, MAXT>, r.threads, \
@@ -414,7 +421,13 @@ static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
 // a CTA of at most 256 threads may have twice the registers of a thread of one of 512
 #define LG_NORM_CTA(U) do { if (r.threads <= 256) LG_NORM(U, 0, 256); else LG_NORM(U, 0, 512); } while (0)
     if (r.group == 8) LG_NORM(1, 8, 128);
-    else if (r.group == 32) { if (r.u == 1) LG_NORM(1, 32, 128); else LG_NORM(2, 32, 128); }
+    else if (r.group == 32) {
+        if (r.u == 1) LG_NORM(1, 32, 128);
+        else if (r.u == 2) LG_NORM(2, 32, 128);
+        else if (r.u == 4) LG_NORM(4, 32, 128);
+        else if (r.u == 8) { if constexpr (VE <= 4) LG_NORM(8, 32, 128); }
+        else { if constexpr (VE <= 2) LG_NORM(16, 32, 128); }
+    }
     else if (r.u == 1) LG_NORM_CTA(1);
     else if (r.u == 2) LG_NORM_CTA(2);
     else if (r.u == 4) LG_NORM_CTA(4);
