@@ -421,7 +421,7 @@ int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t 
                        int64_t n, int64_t weight_stride, int32_t feature_len, void *out, int32_t out_dtype, int64_t out_stride,
                        void *stream);
 /* First error that a kernel of these operators raised on dev_id since the last reset (0: none; LEGION_E_TIMEOUT: a copy or a product
- * inside legion_matmul_rows did not complete within its wait limit, the call's output is not valid).  Waits for `stream`. */
+ * inside legion_matmul_rows or legion_rms_norm_grad did not complete within its wait limit, the call's output is not valid).  Waits for `stream`. */
 int legion_operator_error(int32_t dev_id, void *stream, int32_t *error, int32_t reset);
 
 /* ---- whole batch --------------------------------------------------------------------- */

@@ -1,6 +1,7 @@
 // Products of compressed rows: out[i][j] = sa[i] * sb[j] * sum_k a[i][k] * b[j][k], codes int8 or e4m3, one fp32 scale per row
 // behind the codes.  Nothing is decoded: the codes go to the tensor cores as they lie in memory, the two scales
 // meet the sum in the epilogue.
+#include "async.cuh"
 #include "codec.cuh"
 #include "typed.cuh"
 
@@ -15,25 +16,7 @@ __device__ int32_t g_operator_error = 0;
 
 // ---- PTX ---------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// Waits until the barrier's phase of that parity is over: at most `tries` times 20 microseconds (kTries: two seconds), then false.
-constexpr uint32_t kTries = 100000;
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t tries)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
-        "TRY:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n @p bra DONE;\n sub.u32 n, n, 1;\n setp.gt.s32 q, n, 0;\n @q bra TRY;\n"
-        "DONE:\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok) : "r"(bar), "r"(parity), "r"(tries) : "memory");
-    return ok != 0;
-}
 // PAIR: the barrier may be the other CTA's.
 template <int PAIR>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
@@ -238,7 +221,7 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) tma_store_2d(map, smem_u32(row), q0 + c, p0);
+        if (lane == 0) tma_store_2d(map, shared_addr(row), q0 + c, p0);
     }
 }
 
@@ -298,7 +281,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * BQ);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStagesMax + 4);
     volatile int32_t *gave_up = reinterpret_cast<volatile int32_t *>(tmem_slot + 1);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16;
+    const uint32_t full = shared_addr(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t me = PAIR == 2 ? blockIdx.x & 1 : 0;   // which of the pair
     const int step_p = PAIR == 2 || !P_OUT_COLUMNS ? kPairP : m.step_p;
@@ -314,10 +297,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     auto produce = [&]() {   // the whole warp; one lane issues
         if (block == 0) tile_at(tile, tiles_p, tiles_q, tp, tq);
         if (one_lane()) {
-            uint32_t dst = smem_u32(smem + stage * kStage);
+            uint32_t dst = shared_addr(smem + stage * kStage);
             const uint32_t bar = full_of_first + 8 * stage;
             const int subs = min(kSub, blocks_k - block);
-            if (warp == 4 && me == 0) bar_expect(full + 8 * stage, (uint32_t)subs * sub_bytes * PAIR);   // what all bring
+            if (warp == 4 && me == 0) expect_bytes(full + 8 * stage, (uint32_t)subs * sub_bytes * PAIR);   // what all bring
             for (int i = 0; i < subs; ++i, dst += sub_bytes) {
                 if (warp == 4) tma_2d<PAIR>(dst, &p_map, bar, (block + i) * kTileK, tp * step_p + (int)me * kTileP);
                 else tma_2d<PAIR>(dst + q_at, &q_map, bar, (block + i) * kTileK, tq * BQ + (int)me * (BQ / PAIR));
@@ -336,12 +319,12 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     };
     if (warp == 4) {
         if (lane < S) {
-            bar_init(full + 8 * lane, 1);
-            bar_init(empty + 8 * lane, 1);
+            init_barrier(full + 8 * lane, 1);
+            init_barrier(empty + 8 * lane, 1);
         }
         if (lane < 2) {
-            bar_init(acc_full + 8 * lane, 1);
-            bar_init(acc_empty + 8 * lane, 4 * PAIR);   // the warps that store
+            init_barrier(acc_full + 8 * lane, 1);
+            init_barrier(acc_empty + 8 * lane, 4 * PAIR);   // the warps that store
         }
         if (lane == 0) *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -349,10 +332,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     }
     if (warp == 5) {
         if (PAIR == 2) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(tmem_slot)), "r"(tmem_columns(BQ)) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         }
     }
@@ -365,15 +348,15 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
 
     if (warp == 4 || warp == 6) {
         if (PAIR == 2) full_of_first = in_first_cta(full);
-        uint32_t tries = kTries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
+        uint32_t tries = kWaitTries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
         while (tile < tiles) {
-            if (!bar_wait(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
+            if (!wait_barrier(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
             if (__any_sync(kFull, tries == 0)) break;
             produce();
         }
         // the last products have let go of every stage: nothing signals here any more
         for (int i = 0; i < S; ++i) {
-            if (!bar_wait(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
+            if (!wait_barrier(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
             if (++stage == S) {
                 stage = 0;
                 ++round;
@@ -388,17 +371,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             // The whole warp walks through the stages and one lane of it issues: what the products are issued with stays uniform
             // (issued from a lane on a path of its own, four products took 650 clocks, more than the tensor cores need for 256 x 256).
             constexpr uint32_t idesc = instruction_desc<CODEC, kPairP, BQ>();
-            const uint64_t first = operand_desc(smem_u32(smem));
+            const uint64_t first = operand_desc(shared_addr(smem));
             const uint32_t stage16 = (uint32_t)kStage >> 4, sub16 = sub_bytes >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
             int s = 0, turn = 0;
-            uint32_t around = 0, tries = kTries;
+            uint32_t around = 0, tries = kWaitTries;
             for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
-                if (!bar_wait(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
+                if (!wait_barrier(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
                 fence_after();
                 const uint32_t acc = tmem + a * BQ;
                 for (int kb = 0; kb < blocks_k; kb += kSub) {
-                    if (!bar_wait(full + 8 * s, around & 1, tries)) tries = 0;
+                    if (!wait_barrier(full + 8 * s, around & 1, tries)) tries = 0;
                     const uint64_t dp = first + (uint32_t)s * stage16;
                     const int left = m.k - kb * kTileK;   // 32 codes a product; the last block has as many as the rows reach into
                     if (one_lane()) {
@@ -436,7 +419,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 qs[i] = q < m.q_n ? *reinterpret_cast<const float *>(m.q_rows + (int64_t)q * m.q_stride + m.k) : 0.0f;
             }
             const float ps = mine ? *reinterpret_cast<const float *>(m.p_rows + (int64_t)p * m.p_stride + m.k) : 0.0f;
-            if (!bar_wait(acc_full + 8 * a, (turn >> 1) & 1, kTries)) *gave_up = 1;
+            if (!wait_barrier(acc_full + 8 * a, (turn >> 1) & 1, kWaitTries)) *gave_up = 1;
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
             const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
@@ -562,18 +545,6 @@ static EncodeTiled encode_tiled()
             fn = (EncodeTiled)p;
     }
     return fn;
-}
-
-// What a kernel's launch asks for once per device: more than 48 KB of shared memory.
-static int allow_smem(const void *kernel, int bytes, bool *done)
-{
-    int dev = 0;
-    LG_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !done[dev]) {
-        LG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        if (dev >= 0 && dev < 64) done[dev] = true;
-    }
-    return LEGION_OK;
 }
 
 // k codes of n rows; what a box reaches beyond them (the scales among it) arrives as zeros
@@ -727,11 +698,19 @@ extern "C" int legion_operator_error(int32_t dev_id, void *stream, int32_t *erro
     LG_ARG(error != nullptr, "error is NULL");
     const OnDevice on(dev_id);
     LG_CUDA(on.err);
-    void *word = nullptr;
-    LG_CUDA(cudaGetSymbolAddress(&word, g_operator_error));
+    *error = 0;
     cudaStream_t s = (cudaStream_t)stream;
-    LG_CUDA(cudaMemcpyAsync(error, word, 4, cudaMemcpyDeviceToHost, s));
-    if (reset) LG_CUDA(cudaMemsetAsync(word, 0, 4, s));
-    LG_CUDA(cudaStreamSynchronize(s));
+    for (int k = 0; k < 2; ++k) {
+        void *word = nullptr;
+        int32_t found = 0;
+        LG_CUDA(k == 0 ? cudaGetSymbolAddress(&word, g_operator_error) : norm_error_word(&word));
+        LG_CUDA(cudaMemcpyAsync(&found, word, 4, cudaMemcpyDeviceToHost, s));
+        LG_CUDA(cudaStreamSynchronize(s));
+        if (reset && found != 0) {
+            LG_CUDA(cudaMemsetAsync(word, 0, 4, s));
+            LG_CUDA(cudaStreamSynchronize(s));
+        }
+        if (*error == 0) *error = found;
+    }
     return LEGION_OK;
 }

@@ -8,12 +8,17 @@
 // the sums to the stores.  s is positive and rounding is monotone, so max |y| is s * max |h * w| to the bit, and the norm
 // and the codec share one reduction.  Sums are fp32, h is kept in fp32 until y is rounded; what
 // residual_out receives is h rounded once.  What bounds all of it is HBM.
+#include "async.cuh"
 #include "codec.cuh"
 #include "typed.cuh"
 
 namespace legion {
 
 static constexpr unsigned kFull = 0xFFFFFFFFu;
+
+__device__ int32_t g_norm_error = 0;
+__device__ __forceinline__ void raise_operator_error() { atomicCAS(&g_norm_error, 0, LEGION_E_TIMEOUT); }
+cudaError_t norm_error_word(void **word) { return cudaGetSymbolAddress(word, g_norm_error); }
 
 // Sum and, WITH_MAX, NaN-keeping maximum over the threads of a row.  GROUP lanes of a warp, or (0) the CTA.
 template <int GROUP>
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
             }
         }
     };
-    constexpr bool kAhead = U * VE <= 16 || GROUP == 32;   // wider threads of a CTA have no registers for it
+    constexpr bool kAhead = U * VE <= 16 || GROUP == 32 || sizeof(T) == 2;   // wider threads of a CTA have no registers for it
     const int64_t step = (int64_t)gridDim.x * per_cta;
     if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
     float w[U][VE];
@@ -203,6 +208,9 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
     }
 }
 
+constexpr int kStreamStages = 8;
+constexpr int kStreamSmem = 216 * 1024;   // of an SM, for rows on their way
+
 struct NormGradParams {
     const void *grad_out, *x, *grad_residual, *weight;
     void *grad_x;
@@ -218,6 +226,7 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
     __shared__ float smem[128];
     __shared__ float cross[GROUP == 0 ? 1 : 128 * U * VE];
     RowReduce<GROUP> reduce(smem);
+    cudaTriggerProgrammaticLaunchCompletion();
     const int width = GROUP == 0 ? blockDim.x : GROUP;
     const int t = GROUP == 0 ? threadIdx.x : threadIdx.x & (GROUP - 1);
     const int per_cta = GROUP == 0 ? 1 : 128 / (GROUP == 0 ? 1 : GROUP);
@@ -237,7 +246,8 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
             }
         }
     };
-    constexpr bool kAhead = U * VE <= 16 || GROUP == 32;   // wider threads of a CTA have no registers for it
+    // wider threads have no registers for it (12371 rows of 602 fp32: 51 us with it, 32 without)
+    constexpr bool kAhead = U * VE * (int)sizeof(T) <= 64 && MAXT <= 256;
     const int64_t step = (int64_t)gridDim.x * per_cta;
     if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
     float w[U][VE], dw[U][VE];
@@ -311,22 +321,129 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
     }
 }
 
-// Columns of the CTAs' shares added: 32 columns a CTA, 32 threads a column, one fixed order.
+// The same for long rows on 16-byte boundaries, where there are many: one thread has the copy engine bring whole rows into shared memory,
+// `stages` rows ahead, so that what is on its way does not depend on registers.  A stage is free again when the threads
+// have met in the row's reduction: by then all of them have read their part of it.
+// Measured, 16384 rows of 2048 bf16 (268 MB): 64 us with the next row in registers, 72 without it.
+template <typename T, int U, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_grad_stream_kernel(NormGradParams p, int stages)
+{
+    constexpr int VE = 16 / (int)sizeof(T);
+    extern __shared__ __align__(128) uint8_t rows[];   // [stage][x, grad_out, grad_residual][row]
+    __shared__ float smem[128];
+    __shared__ uint64_t bars[kStreamStages];
+    RowReduce<0> reduce(smem);
+    const int t = threadIdx.x, width = blockDim.x;
+    const uint32_t row_bytes = (uint32_t)p.dim * sizeof(T);
+    const int arrays = p.grad_residual != nullptr ? 3 : 2;
+    auto bring = [&](int64_t row, int stage) {   // one thread
+        const uint32_t bar = shared_addr(&bars[stage]), dst = shared_addr(rows) + stage * arrays * row_bytes;
+        expect_bytes(bar, arrays * row_bytes);
+        bulk_copy(dst, static_cast<const T *>(p.x) + row * p.x_stride, row_bytes, bar);
+        bulk_copy(dst + row_bytes, static_cast<const T *>(p.grad_out) + row * p.grad_stride, row_bytes, bar);
+        if (arrays == 3) bulk_copy(dst + 2 * row_bytes, static_cast<const T *>(p.grad_residual) + row * p.grad_residual_stride, row_bytes, bar);
+    };
+    const int64_t step = gridDim.x;
+    cudaTriggerProgrammaticLaunchCompletion();
+    if (t == 0) {
+        for (int s = 0; s < stages; ++s) init_barrier(shared_addr(&bars[s]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int s = 0; s < stages; ++s)
+            if (blockIdx.x + s * step < p.n) bring(blockIdx.x + s * step, s);
+    }
+    float w[U][VE], dw[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, w[u]);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) dw[u][i] = 0.0f;
+    }
+    __syncthreads();
+    int stage = 0;
+    uint32_t phase = 0, tries = kWaitTries;
+    for (int64_t row = blockIdx.x; row < p.n; row += step) {
+        if (!wait_barrier(shared_addr(&bars[stage]), phase, tries)) tries = 0;   // given up: the rest is not waited for, the error is kept
+        const uint8_t *src = rows + (size_t)stage * arrays * row_bytes;
+        Vec<T, VE> h[U], dy[U], r[U];
+        float square = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            h[u].zero();
+            dy[u].zero();
+            r[u].zero();
+            if (col < p.dim) {
+                h[u].load(reinterpret_cast<const T *>(src) + col);
+                dy[u].load(reinterpret_cast<const T *>(src + row_bytes) + col);
+                if (arrays == 3) r[u].load(reinterpret_cast<const T *>(src + 2 * row_bytes) + col);
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float a = h[u].get(i);
+                square = fmaf(a, a, square);
+                dot = fmaf(dy[u].get(i) * w[u][i], a, dot);
+            }
+        }
+        reduce.two(square, dot, false);
+        if (t == 0 && row + stages * step < p.n && tries != 0) bring(row + stages * step, stage);
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+        const float s = 1.0f / sqrtf(square / (float)p.dim + p.eps);
+        const float k = s * s * s * (dot / (float)p.dim);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int col = (t + u * width) * VE;
+            if (col >= p.dim) continue;
+            float dx[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float a = h[u].get(i), g = dy[u].get(i);
+                dx[i] = s * (g * w[u][i]) - a * k + r[u].get(i);
+                dw[u][i] = fmaf(g, a * s, dw[u][i]);
+            }
+            Vec<T, VE> o;
+            o.set(dx);
+            o.store(static_cast<T *>(p.grad_x) + row * p.grad_x_stride + col);
+        }
+    }
+    float *part = p.part + (int64_t)blockIdx.x * p.dim;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int col = (t + u * width) * VE;
+        if (col >= p.dim) continue;
+        Vec<float, VE> o;
+        o.set(dw[u]);
+        o.store(part + col);
+    }
+    if (tries == 0) {
+        raise_operator_error();
+        if (t == 0)   // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
+            for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
+        __syncthreads();
+    }
+}
+
+// Columns of the CTAs' shares added: 16 columns a CTA, 64 threads a column, one fixed order.
 __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float *__restrict__ part, int parts, int dim, void *out, int dtype)
 {
-    __shared__ float s[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + x;
+    __shared__ float s[64][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + x;
+    cudaGridDependencySynchronize();
     float sum = 0.0f;
     if (col < dim)
-#pragma unroll 8
-        for (int g = y; g < parts; g += 32) sum += part[(int64_t)g * dim + col];
+#pragma unroll 10
+        for (int g = y; g < parts; g += 64) sum += part[(int64_t)g * dim + col];
     s[y][x] = sum;
     __syncthreads();
-    sum = s[x][y];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (warp >= 16) return;
+    sum = s[lane][warp] + s[lane + 32][warp];
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-    if (x == 0 && blockIdx.x * 32 + y < dim) store_any(out, dtype, blockIdx.x * 32 + y, sum);
+    if (lane == 0 && blockIdx.x * 16 + warp < dim) store_any(out, dtype, blockIdx.x * 16 + warp, sum);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
@@ -410,9 +527,47 @@ static int launch_norm_codec(cudaStream_t s, const NormParams &p, int codec, int
     return launch_norm_ve<T, LEGION_CODEC_E4M3>(s, p, ve);
 }
 
+template <typename T, int U, int MAXT>
+static int launch_norm_grad_stream(cudaStream_t s, const NormGradParams &p, int threads, int *parts)
+{
+    const void *kernel = (const void *)norm_grad_stream_kernel<T, U, MAXT>;
+    static bool allowed[64];
+    const int rc = allow_smem(kernel, kStreamSmem, allowed);
+    if (rc != LEGION_OK) return rc;
+    const int stage = (p.grad_residual != nullptr ? 3 : 2) * p.dim * (int)sizeof(T);
+    // CTAs by their registers; each SM's shared memory is shared out among them, two stages a CTA at least
+    int fit = 0;
+    LG_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, 0));
+    if (fit > kGradCtas / kSms) fit = kGradCtas / kSms;
+    while (fit > 1 && kStreamSmem / fit < 2 * stage) --fit;
+    int stages = kStreamSmem / (fit < 1 ? 1 : fit) / stage;
+    if (stages > kStreamStages) stages = kStreamStages;
+    const int64_t most = (int64_t)(fit < 1 ? 1 : fit) * kSms;
+    *parts = (int)(p.n < most ? p.n : most);
+    norm_grad_stream_kernel<T, U, MAXT><<<*parts, threads, stages * stage, s>>>(p, stages);
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}
+
 template <typename T, int VE>
 static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
 {
+    if constexpr (VE * sizeof(T) == 16) {
+        const int64_t bytes = (int64_t)p.dim * sizeof(T), stage = (p.grad_residual != nullptr ? 3 : 2) * bytes;
+        const int vecs = p.dim / VE;
+        // (20000 rows of 2048 bytes: 47 us like this, 34 by a warp each; 16384 of 4096: 61 and 64; 4000 of 16 KB: 58 and 88)
+        if (bytes >= 4096 && p.n >= 4 * kSms && 2 * stage <= kStreamSmem) {
+            int u = 1;
+            while (u < 4 && (vecs + u - 1) / u > 256) u *= 2;
+            const int threads = ((vecs + u - 1) / u + 31) / 32 * 32;
+            if (threads <= 256) {
+                if (u == 1) return launch_norm_grad_stream<T, 1, 256>(s, p, threads, parts);
+                if (u == 2) return launch_norm_grad_stream<T, 2, 256>(s, p, threads, parts);
+                return launch_norm_grad_stream<T, 4, 256>(s, p, threads, parts);
+            }
+            if (threads <= 512) return launch_norm_grad_stream<T, 4, 512>(s, p, threads, parts);
+        }
+    }
     const RowShape r = row_shape(p.dim / VE, VE, p.n);
     const int64_t need = (p.n + r.per_cta - 1) / r.per_cta;
 #define LG_NORM(U, GROUP, MAXT)                                                                                                    \
@@ -547,7 +702,16 @@ extern "C" int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_
     else if (dtype == LEGION_F16) rc = launch_norm_grad_ve<__half>(s, p, ve, &parts);
     else rc = launch_norm_grad_ve<__nv_bfloat16>(s, p, ve, &parts);
     if (rc != LEGION_OK) return rc;
-    norm_weight_grad_kernel<<<(dim + 31) / 32, 1024, 0, s>>>((const float *)workspace, parts, dim, grad_weight, grad_weight_dtype);
-    LG_LAUNCH_CHECK();
+    // as a dependent of the launch before it, which it may overlap up to its cudaGridDependencySynchronize
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(dim + 15) / 16);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    LG_CUDA(cudaLaunchKernelEx(&cfg, norm_weight_grad_kernel, (const float *)workspace, parts, (int)dim, grad_weight, (int)grad_weight_dtype));
     return LEGION_OK;
 }

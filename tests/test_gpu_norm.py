@@ -219,3 +219,29 @@ def test_no_rows_and_refusals():
                 lambda: L.rms_norm_grad(0, x, x, w, x, dw.half(), torch.zeros(1 << 12, device="cuda"))):
         with pytest.raises(L.LegionError):
             bad()
+
+
+@pytest.mark.parametrize("n,dim,dtype", [(592, 1024, "bf16"), (593, 4096, "bf16"), (1000, 8192, "f16"), (700, 2052, "f32"), (2000, 512, "f32"), (595, 6000, "f32"),
+                                         (600, 16384, "bf16"), (3000, 1032, "f16")])
+@pytest.mark.parametrize("residual", [False, True])
+def test_gradient_of_many_long_rows(n, dim, dtype, residual):
+    """Rows that the copy engine brings: around the smallest number of them, rows per CTA that differ, one stage more and less."""
+    import torch
+    t = _types()[dtype]
+    x, w, r = _inputs(n, dim, t, torch.float32, residual, 16 // t.itemsize, 0, 5)
+    dy = torch.randn(n, dim, device="cuda").to(t)
+    dx, dw = torch.empty_like(dy), torch.zeros(dim, device="cuda")
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda").fill_(0xFF)
+    L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 1e-5, r)
+    h, g = x.double(), dy.double() * w.double()
+    s = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+    first, second = s * g, h * s ** 3 * (g * h).mean(1, keepdim=True)
+    extra = r.double() if residual else torch.zeros_like(h)
+    mag = first.abs() + h.abs() * s ** 3 * (g * h).abs().mean(1, keepdim=True) + extra.abs()
+    _close(dx, first - second + extra, mag * (130 * U32))
+    terms = dy.double() * h * s
+    _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
+    assert L.operator_error(0) == 0
+    dw2 = torch.zeros_like(dw)
+    L.rms_norm_grad(0, dy, x, w, dy, dw2, ws, 1e-5, r)   # in place
+    assert torch.equal(dy, dx) and torch.equal(dw, dw2)
