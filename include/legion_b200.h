@@ -360,7 +360,7 @@ int legion_gather_rows_noalloc(void *stream, int32_t dev_id, const int32_t *ids_
  * not share a workspace or an output.  Rows are rows of dim elements; strides are in elements (compressed rows: in bytes) and may be
  * longer than the row; what lies between rows is neither read nor written.  Addresses are multiples of the element's size; rows
  * whose addresses, strides and length are multiples of 16 bytes move by the widest loads.  Results do not depend on the order in
- * which the GPU runs its blocks: the same call gives the same bits. */
+ * which the GPU runs its blocks: the same call on rows that lie the same way in memory gives the same bits. */
 #define LEGION_F32 0
 #define LEGION_F16 1
 #define LEGION_BF16 2

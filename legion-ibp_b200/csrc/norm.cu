@@ -12,6 +12,8 @@
 #include "codec.cuh"
 #include "typed.cuh"
 
+#include <utility>
+
 namespace legion {
 
 static constexpr unsigned kFull = 0xFFFFFFFFu;
@@ -205,6 +207,96 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(NormParams p)
         }
         const int tail = (int)((code_row_bytes(p.dim) - p.dim) >> 2);
         if (t < tail) reinterpret_cast<uint32_t *>(dst + p.dim)[t] = t == 0 ? __float_as_uint(scale) : 0u;
+    }
+}
+
+// Long rows of an odd number of elements, where all operands' rows lie alike: vectors are those of memory, not of the row.  A row begins `shift` elements into its first vector; whole vectors are moved as such, the two at the ends
+// element by element.  Which weight meets which element of a vector then changes from row to row: weights lie in shared
+// memory, column j at [j % VE][j / VE], where the lanes of an access hit different banks whatever the shift.
+// Measured, with residual: 8192 rows of 4097 bf16 109 us, 291 element by element; 4000 of 4097 fp32 75 us, 250.  Rows that a warp holds are
+// better off with elements (20000 of 603 fp16: 45 us like this, 35), and so are rows on 4-byte boundaries with vectors of four bytes (8192 of
+// 4098 bf16: 109 us like this, 82).
+template <typename T, int U>
+struct Framed {
+    static constexpr int VE = 16 / (int)sizeof(T);
+    int t, width, dim, pitch;
+    __device__ __forceinline__ int first(int u, int shift) const { return (t + u * width) * VE - shift; }   // column of the vector's first element
+    __device__ __forceinline__ int at(int u, int i, int shift) const   // of element i's column in a table laid out as above
+    {
+        const int v = t + u * width, q = i - shift;
+        return q < 0 ? (q + VE) * pitch + v - 1 : q * pitch + v;
+    }
+    __device__ __forceinline__ bool has(int u, int i, int shift) const { return (unsigned)(first(u, shift) + i) < (unsigned)dim; }
+    __device__ __forceinline__ void load(const T *row, int shift, Vec<T, VE> *v) const
+    {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = first(u, shift);
+            v[u].zero();
+            if (c >= 0 && c + VE <= dim) {
+                v[u].load(row + c);
+            } else if (c + VE > 0 && c < dim) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (has(u, i, shift)) v[u].e[i] = row[c + i];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *row, int shift, int u, const float *x) const
+    {
+        const int c = first(u, shift);
+        Vec<T, VE> v;
+        v.set(x);
+        if (c >= 0 && c + VE <= dim) {
+            v.store(row + c);
+        } else if (c + VE > 0 && c < dim) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (has(u, i, shift)) row[c + i] = v.e[i];
+        }
+    }
+};
+constexpr int kFramedThreads = 544;   // 16384 elements, four vectors of eight or eight of four a thread, and the ends
+// words of such a table
+__host__ __device__ __forceinline__ int framed_pitch(int dim, int ve) { return dim / ve + 2; }
+
+template <typename T, int U>
+__global__ void __launch_bounds__(kFramedThreads) norm_framed_kernel(NormParams p)
+{
+    constexpr int VE = 16 / (int)sizeof(T);
+    extern __shared__ float table[];
+    __shared__ float smem[128];
+    RowReduce<0> reduce(smem);
+    const Framed<T, U> f{ (int)threadIdx.x, (int)blockDim.x, p.dim, framed_pitch(p.dim, VE) };
+    for (int j = threadIdx.x; j < p.dim; j += blockDim.x) table[(j % VE) * f.pitch + j / VE] = load_any(p.weight, p.weight_dtype, j);
+    __syncthreads();
+    for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
+        const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+        const int shift = (int)((uintptr_t)x / sizeof(T) % VE);
+        Vec<T, VE> a[U], r[U];
+        f.load(x, shift, a);
+        if (p.residual != nullptr) f.load(static_cast<const T *>(p.residual) + row * p.residual_stride, shift, r);
+        float h[U][VE];
+        float sum = 0.0f, unused = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                h[u][i] = a[u].get(i);
+                if (p.residual != nullptr) h[u][i] += r[u].get(i);
+                sum = fmaf(h[u][i], h[u][i], sum);
+            }
+            if (p.residual_out != nullptr) f.store(static_cast<T *>(p.residual_out) + row * p.residual_out_stride, shift, u, h[u]);
+        }
+        reduce.two(sum, unused, false);
+        const float s = 1.0f / sqrtf(sum / (float)p.dim + p.eps);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (f.has(u, i, shift)) h[u][i] = h[u][i] * table[f.at(u, i, shift)] * s;
+            f.store(static_cast<T *>(p.out) + row * p.out_stride, shift, u, h[u]);
+        }
     }
 }
 
@@ -468,13 +560,51 @@ static RowShape row_shape(int vecs, int ve, int64_t n)
 }
 
 // CTAs of a kernel that loops over rows: as many as are on the chip at one time (at most `per_sm` a SM), so that none starts late.
-static unsigned resident(int64_t need, const void *kernel, int threads, int per_sm)
+static unsigned resident(int64_t need, const void *kernel, int threads, int per_sm, int smem = 0)
 {
     if (need <= kSms) return (unsigned)need;
     int fit = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, 0) != cudaSuccess || fit < 1) fit = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, smem) != cudaSuccess || fit < 1) fit = 1;
     if (fit > per_sm) fit = per_sm;
     return (unsigned)(need < (int64_t)fit * kSms ? need : (int64_t)fit * kSms);
+}
+
+template <typename T, int U>
+static int go_framed(cudaStream_t s, const NormParams &p, int threads)
+{
+    constexpr int VE = 16 / (int)sizeof(T);
+    const void *kernel = (const void *)norm_framed_kernel<T, U>;
+    const int smem = 4 * VE * framed_pitch(p.dim, VE);
+    static bool allowed[64];
+    const int rc = allow_smem(kernel, 4 * VE * framed_pitch(LEGION_NORM_MAX_DIM, VE), allowed);
+    if (rc != LEGION_OK) return rc;
+    norm_framed_kernel<T, U><<<resident(p.n, kernel, threads, 16, smem), threads, smem, s>>>(p);
+    LG_LAUNCH_CHECK();
+    return LEGION_OK;
+}
+
+template <typename T>
+static int launch_framed(cudaStream_t s, const NormParams &p)
+{
+    constexpr int VE = 16 / (int)sizeof(T);
+    const int vecs = p.dim / VE + 2;
+    int u = 1;
+    while (u * VE < 32 && (vecs + u - 1) / u > 256) u *= 2;
+    const int threads = ((vecs + u - 1) / u + 31) / 32 * 32;
+    if (u == 1) return go_framed<T, 1>(s, p, threads);
+    if (u == 2) return go_framed<T, 2>(s, p, threads);
+    if constexpr (VE == 8) return go_framed<T, 4>(s, p, threads);
+    else return u == 4 ? go_framed<T, 4>(s, p, threads) : go_framed<T, 8>(s, p, threads);
+}
+
+// Whether all rows of the operands lie alike in 16-byte vectors.
+static bool lie_alike(int dtype, std::initializer_list<std::pair<const void *, int64_t>> rows)
+{
+    const auto &first = *rows.begin();
+    for (const auto &r : rows)
+        if (r.first != nullptr && (((uintptr_t)r.first ^ (uintptr_t)first.first) % 16 != 0 || (r.second - first.second) % (16 / dtype_bytes(dtype)) != 0))
+            return false;
+    return true;
 }
 
 template <typename T, int VE, int CODEC>
@@ -648,6 +778,12 @@ extern "C" int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int
     if (residual_out != nullptr) ve = common_vector(ve, { residual_out_stride, aligned_elements(residual_out, dtype) });
     if (codec == LEGION_CODEC_RAW) ve = common_vector(ve, { out_stride, aligned_elements(out, dtype) });
     cudaStream_t s = (cudaStream_t)stream;
+    if (codec == LEGION_CODEC_RAW && ve == 1 && dim > 1024 && n_rows >= 2 * kSms &&
+        lie_alike(dtype, { { x, x_stride }, { residual, residual_stride }, { out, out_stride }, { residual_out, residual_out_stride } })) {
+        if (dtype == LEGION_F32) return launch_framed<float>(s, p);
+        if (dtype == LEGION_F16) return launch_framed<__half>(s, p);
+        return launch_framed<__nv_bfloat16>(s, p);
+    }
     if (dtype == LEGION_F32) return launch_norm_codec<float>(s, p, codec, ve);
     if (dtype == LEGION_F16) return launch_norm_codec<__half>(s, p, codec, ve);
     return launch_norm_codec<__nv_bfloat16>(s, p, codec, ve);

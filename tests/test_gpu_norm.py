@@ -42,7 +42,7 @@ def test_norm(n, dim, dtype, residual):
     for pad, shift, wt in ((0, 0, torch.float32), (8, 8, t), (3, 1, t)):
         x, w, r = _inputs(n, dim, t, wt, residual, pad, shift)
         whole, out = _strided(n, dim, t, pad, shift)
-        total = torch.zeros(n, dim, dtype=t, device="cuda") if residual else None
+        total = _strided(n, dim, t, pad, shift)[1] if residual else None
         L.rms_norm(0, x, w, out, 1e-5, r, total)
         h, y = _exact(x, w, r, 1e-5)
         _close(out, y, y.abs() * (32 * U32))
@@ -127,7 +127,7 @@ def test_gradient(n, dim, dtype, residual):
         _close(dx, first - second + extra, mag * (130 * U32))
         terms = dy.double() * h * s
         _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
-        again, dw2 = torch.empty(n, dim, dtype=t, device="cuda"), torch.zeros_like(dw)
+        again, dw2 = _strided(n, dim, t, pad, shift)[1], torch.zeros_like(dw)
         L.rms_norm_grad(0, dy, x, w, again, dw2, ws, 1e-5, r)
         assert torch.equal(dw, dw2) and torch.equal(dx, again)
     # in place over the gradient that came in
@@ -244,4 +244,46 @@ def test_gradient_of_many_long_rows(n, dim, dtype, residual):
     assert L.operator_error(0) == 0
     dw2 = torch.zeros_like(dw)
     L.rms_norm_grad(0, dy, x, w, dy, dw2, ws, 1e-5, r)   # in place
+    assert torch.equal(dy, dx) and torch.equal(dw, dw2)
+
+
+@pytest.mark.parametrize("n,dim", [(1, 65), (7, 101), (2000, 129), (1300, 255), (600, 602), (50, 1022), (900, 1030), (300, 2047), (296, 1025), (297, 12289), (500, 1027), (700, 4097), (20, 8191), (3, 16383),
+                                   (400, 16382)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (0, 3), (5, 1), (8, 2)])
+def test_rows_that_start_anywhere(n, dim, dtype, pad, shift):
+    """Rows that begin at every place of a 16-byte vector, all operands alike; forward, backward, in place; nothing beside the rows is touched."""
+    import torch
+    t = _types()[dtype]
+    x, w, r = _inputs(n, dim, t, t, True, pad, shift, 2)
+    whole, out = _strided(n, dim, t, pad, shift)
+    wholes, total = _strided(n, dim, t, pad, shift)
+    L.rms_norm(0, x, w, out, 1e-5, r, total)
+    h, y = _exact(x, w, r, 1e-5)
+    _close(out, y, y.abs() * (32 * U32))
+    _close(total, h, h.abs() * U32)
+    for mem in (whole, wholes):
+        rest = mem.clone()
+        torch.as_strided(rest, (n, dim), (dim + pad, 1), shift).fill_(7.0)
+        assert bool((rest == 7.0).all())
+    a = _strided(n, dim, t, pad, shift)[1]
+    a.copy_(x)
+    L.rms_norm(0, a, w, a, 1e-5, r)
+    assert torch.equal(a, out)
+    dy, (mem, dx), dw = _strided(n, dim, t, pad, shift)[1], _strided(n, dim, t, pad, shift), torch.zeros(dim, device="cuda")
+    dy.copy_(torch.randn(n, dim, device="cuda"))
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda").fill_(0xFF)
+    L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 1e-5, r)
+    h, g = x.double(), dy.double() * w.double()
+    s = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+    first, second = s * g, h * s ** 3 * (g * h).mean(1, keepdim=True)
+    mag = first.abs() + h.abs() * s ** 3 * (g * h).abs().mean(1, keepdim=True) + r.double().abs()
+    _close(dx, first - second + r.double(), mag * (130 * U32))
+    terms = dy.double() * h * s
+    _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
+    rest = mem.clone()
+    torch.as_strided(rest, (n, dim), (dim + pad, 1), shift).fill_(7.0)
+    assert bool((rest == 7.0).all())
+    dw2 = torch.zeros_like(dw)
+    L.rms_norm_grad(0, dy, x, w, dy, dw2, ws, 1e-5, r)
     assert torch.equal(dy, dx) and torch.equal(dw, dw2)
