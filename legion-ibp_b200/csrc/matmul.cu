@@ -127,7 +127,7 @@ struct MatmulParams {
     void *out;
     int64_t out_stride;
     int32_t out_dtype;
-    int32_t aligned;  // the output's rows start on multiples of 16 bytes
+    int32_t word;     // the widest word of 16, 8, 4 or 2 bytes that the output's rows start on multiples of
     int32_t stages, stage_bytes, q_at;   // of shared memory; where a stage's rows of Q begin
     int32_t step_p;   // rows of P per CTA and tile: kTileP, or fewer (a multiple of 8) where that gives every SM a tile
 };
@@ -173,22 +173,24 @@ __device__ __forceinline__ void store_one(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void store_one(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-// A lane's row of the tile (P_OUT_COLUMNS: its column of the output) by plain stores.
-template <int CODEC, typename T, int BQ, bool P_OUT_COLUMNS>
-__device__ __forceinline__ void store_lane(uint32_t acc, float ps, const float *qs, int q0, int p, bool mine, const MatmulParams &m)
+// `rows` rows of `cols` values of type T from shared memory (WIDTH values a row, SWIZZLED: 128 bytes with their 16-byte pieces in the
+// order of the TMA swizzle) to rows `stride` apart, by words of type W: consecutive lanes write consecutive words.
+template <typename W, typename T, int WIDTH, bool SWIZZLED>
+__device__ __forceinline__ void write_rows(T *dst, int64_t stride, const uint8_t *src, int rows, int cols)
 {
-    constexpr int N = BQ < 32 ? BQ : 32;
-#pragma unroll 1
-    for (int c = 0; c < BQ && q0 + c < m.q_n; c += N) {
-        float v[N];
-        load_sums<CODEC, N>(acc + c, v);
-        if (!mine) continue;
-        const int left = m.q_n - q0 - c;
-        T *dst = static_cast<T *>(m.out) + (P_OUT_COLUMNS ? (int64_t)(q0 + c) * m.out_stride + p : (int64_t)p * m.out_stride + q0 + c);
-        const int64_t step = P_OUT_COLUMNS ? m.out_stride : 1;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < left) store_one(dst + i * step, v[i] * ps * qs[c + i]);
+    if constexpr (sizeof(W) >= sizeof(T)) {
+        constexpr int kPer = (int)(sizeof(W) / sizeof(T)), kWords = WIDTH / kPer, kBytes = WIDTH * (int)sizeof(T);
+#pragma unroll 8
+        for (int i = threadIdx.x & 31; i < rows * kWords; i += 32) {
+            const int r = i / kWords, w = i % kWords, at = w * (int)sizeof(W);
+            const uint8_t *s = src + r * kBytes + (SWIZZLED ? ((at / 16) ^ (r & 7)) * 16 + at % 16 : at);
+            T *d = dst + r * stride + w * kPer;
+            if ((w + 1) * kPer <= cols) {
+                *reinterpret_cast<W *>(d) = *reinterpret_cast<const W *>(s);
+            } else {
+                for (int j = 0; j < kPer && w * kPer + j < cols; ++j) d[j] = reinterpret_cast<const T *>(s)[j];
+            }
+        }
     }
 }
 
@@ -219,18 +221,29 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
                 o.store(reinterpret_cast<T *>(row + (((half + i) / kPer16) ^ (lane & 7)) * 16));
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) tma_store_2d(map, shared_addr(row), q0 + c, p0);
+        if (m.word == 16) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map, shared_addr(row), q0 + c, p0);
+        } else {   // rows that TMA cannot address: the lanes write along them, in words that the rows start on
+            __syncwarp();
+            const int rows = min(32, m.p_n - p0), cols = min(kCols, m.q_n - q0 - c);
+            T *dst = static_cast<T *>(m.out) + (int64_t)p0 * m.out_stride + q0 + c;
+            const uint8_t *src = row - lane * 128;
+            if (m.word == 8) write_rows<uint2, T, kCols, true>(dst, m.out_stride, src, rows, cols);
+            else if (m.word == 4) write_rows<uint32_t, T, kCols, true>(dst, m.out_stride, src, rows, cols);
+            else write_rows<uint16_t, T, kCols, true>(dst, m.out_stride, src, rows, cols);
+            __syncwarp();
+        }
     }
 }
 
-// The same for P_OUT_COLUMNS where the output's rows start on multiples of 16 bytes: 32 x 32 sums change places in shared memory, so
-// that a lane stores 16 bytes of a row of the output (2-byte stores took 66 clocks each: 4000 clocks for 64 rows).
+// The same for P_OUT_COLUMNS: 32 x 32 sums change places in shared memory, so that the lanes write along the rows of the output (2-byte
+// stores took 66 clocks each: 4000 clocks for 64 rows).
 template <int CODEC, typename T, int BQ>
 __device__ __forceinline__ void store_turned(uint32_t acc, float ps, const float *qs, uint8_t *buffer, int q0, int p0, int valid, const MatmulParams &m)
 {
-    constexpr int N = BQ < 32 ? BQ : 32, kPer16 = 16 / (int)sizeof(T), kPieces = 32 / kPer16;
+    constexpr int N = BQ < 32 ? BQ : 32;
     const int lane = threadIdx.x & 31;
     T *mine = reinterpret_cast<T *>(buffer);
 #pragma unroll 1
@@ -242,16 +255,11 @@ __device__ __forceinline__ void store_turned(uint32_t acc, float ps, const float
         for (int i = 0; i < N; ++i) store_one(mine + i * 32 + lane, v[i] * ps * qs[c + i]);
         __syncwarp();
         const int rows = min(N, m.q_n - q0 - c);
-        for (int i = lane; i < rows * kPieces; i += 32) {
-            const int row = i / kPieces, piece = i % kPieces;
-            T *dst = static_cast<T *>(m.out) + (int64_t)(q0 + c + row) * m.out_stride + p0 + piece * kPer16;
-            const T *src = mine + row * 32 + piece * kPer16;
-            if ((piece + 1) * kPer16 <= valid) {
-                *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
-            } else {
-                for (int j = 0; j < kPer16 && piece * kPer16 + j < valid; ++j) dst[j] = src[j];
-            }
-        }
+        T *dst = static_cast<T *>(m.out) + (int64_t)(q0 + c) * m.out_stride + p0;
+        if (m.word == 16) write_rows<uint4, T, 32, false>(dst, m.out_stride, buffer, rows, valid);
+        else if (m.word == 8) write_rows<uint2, T, 32, false>(dst, m.out_stride, buffer, rows, valid);
+        else if (m.word == 4) write_rows<uint32_t, T, 32, false>(dst, m.out_stride, buffer, rows, valid);
+        else write_rows<uint16_t, T, 32, false>(dst, m.out_stride, buffer, rows, valid);
     }
 }
 
@@ -260,7 +268,8 @@ __device__ __forceinline__ void store_turned(uint32_t acc, float ps, const float
 // PAIR 2: two CTAs take tiles of 256 x BQ together: each loads its 128 rows of P and half of the rows of Q, the first one issues
 // the products of both, each holds and stores the sums of its own rows of P.
 // The output leaves by TMA: a warp writes 128 bytes of each of its 32 rows to shared memory (in the swizzle that the store
-// undoes, so that lanes hit different banks); rows that TMA cannot address are stored by the lanes themselves.
+// undoes, so that lanes hit different banks); rows that TMA cannot address are written by the lanes along the rows (every lane along its
+// own row, 510 x 7548 bf16 took 47 us).
 // P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.  A tile then has step_p rows of P,
 // as many as spread the weights over all SMs.  The products read 128 rows all the same: what lies behind the tile's rows in shared
 // memory reaches nobody's sums but those of rows that are not stored.
@@ -424,21 +433,15 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             fence_after();
             const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
             uint8_t *buffer = out_smem + warp * kOut * kOutBytes;
-            if (m.aligned && P_OUT_COLUMNS) {
+            if constexpr (P_OUT_COLUMNS) {
                 const int p0 = p - lane, valid = min(step_p - warp * 32, m.p_n - p0);
                 if (m.out_dtype == LEGION_F32) store_turned<CODEC, float, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
                 else if (m.out_dtype == LEGION_F16) store_turned<CODEC, __half, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
                 else store_turned<CODEC, __nv_bfloat16, BQ>(acc, ps, qs, buffer, tq * BQ, p0, valid, m);
-            } else if (m.aligned) {
-                if constexpr (!P_OUT_COLUMNS) {
-                    if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
-                    else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
-                    else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
-                }
             } else {
-                if (m.out_dtype == LEGION_F32) store_lane<CODEC, float, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
-                else if (m.out_dtype == LEGION_F16) store_lane<CODEC, __half, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
-                else store_lane<CODEC, __nv_bfloat16, BQ, P_OUT_COLUMNS>(acc, ps, qs, tq * BQ, p, mine, m);
+                if (m.out_dtype == LEGION_F32) store_tile<CODEC, float, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
+                else if (m.out_dtype == LEGION_F16) store_tile<CODEC, __half, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
+                else store_tile<CODEC, __nv_bfloat16, BQ, kOut>(acc, ps, qs, buffer, &out_map, tq * BQ, p - lane, m, copies);
             }
             fence_before();
             __syncwarp();
@@ -594,8 +597,9 @@ static int launch_tiles(cudaStream_t s, MatmulParams m)
     if (rc != LEGION_OK) return rc;
     CUtensorMap out_map;
     memset(&out_map, 0, sizeof(out_map));
-    m.aligned = (uintptr_t)m.out % 16 == 0 && m.out_stride * dtype_bytes(m.out_dtype) % 16 == 0;
-    if (m.aligned && !P_OUT_COLUMNS) rc = make_out_map(&out_map, m);
+    m.word = 16;
+    while (((uintptr_t)m.out | (uintptr_t)(m.out_stride * dtype_bytes(m.out_dtype))) % m.word != 0) m.word /= 2;
+    if (m.word == 16 && !P_OUT_COLUMNS) rc = make_out_map(&out_map, m);
     if (rc != LEGION_OK) return rc;
     // As many stages as there is room for: what is on its way is what hides the latency of memory.
     m.q_at = m.step_p * kTileK;
