@@ -355,10 +355,11 @@ int legion_gather_rows_noalloc(void *stream, int32_t dev_id, const int32_t *ids_
 
 /* Operators that a model needs next to the rows served above: lookup of learned rows with its gradient, RMS norm
  * with its gradient, and products of compressed rows.  They work on device memory of dev_id, in the order of `stream`,
- * allocate nothing, keep nothing between calls, do not synchronise, may be captured into a CUDA graph, and leave the calling
- * thread's current device as it was.  Calls on different streams may run at the same time as long as they do
+ * allocate nothing, keep nothing between calls, do not synchronise, may be captured into a CUDA graph (make a first call on the device
+ * before the capture, as code is loaded with it), and leave the calling thread's current device as it was.  Calls on different streams may run at the same time as long as they do
  * not share a workspace or an output.  Rows are rows of dim elements; strides are in elements (compressed rows: in bytes) and may be
- * longer than the row; what lies between rows is neither read nor written.  Addresses are multiples of the element's size; rows
+ * longer than the row; what lies between rows is neither read nor written, and an output may share memory with an input only where
+ * a call says so.  Addresses are multiples of the element's size; rows
  * whose addresses, strides and length are multiples of 16 bytes move by the widest loads.  Results do not depend on the order in
  * which the GPU runs its blocks: the same call on rows that lie the same way in memory gives the same bits. */
 #define LEGION_F32 0
@@ -398,7 +399,7 @@ int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32_t id_bytes
  * out receives compressed rows, out_stride bytes apart (a multiple of 16): dim codes, an fp32 scale, zeros up to a multiple of 16
  * bytes, exactly what legion_quantize_table makes of the fp32 rows (dim % 4 == 0).  out and residual_out may be x or residual
  * themselves (same address and stride), but not each other; other overlaps are not allowed.  h and its squares are fp32: a
- * row whose squares sum to more than 3.4e38 has an infinite mean. */
+ * row whose squares sum to more than 3.4e38 has an infinite mean.  With eps 0 a row of zeros has no finite norm: its result is NaN. */
 int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stride, const void *residual,
                     int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim,
                     int32_t codec, void *out, int64_t out_stride, void *residual_out, int64_t residual_out_stride, void *stream);

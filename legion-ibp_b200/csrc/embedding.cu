@@ -1145,6 +1145,11 @@ extern "C" int legion_embedding_lookup(int32_t dev_id, const void *table, int32_
     if (rc != LEGION_OK) return rc;
     LG_ROWS(table, table_dtype, dim, table_stride, n_nodes, "table");
     LG_ROWS(out, out_dtype, dim, out_stride, n_ids, "out");
+    LG_ARG(n_ids == 0 || out != table, "out must not be the table");
+    if (n_ids * dim > (1ll << 40)) {
+        set_error("legion_embedding_lookup: %lld rows of %d elements are above the limit of 2^40 elements", (long long)n_ids, dim);
+        return LEGION_E_LIMIT;
+    }
     if (n_ids == 0) return LEGION_OK;
     const OnDevice on(dev_id);
     LG_CUDA(on.err);
@@ -1186,6 +1191,7 @@ extern "C" int legion_embedding_grad(int32_t dev_id, const void *ids, int32_t id
     if (rc != LEGION_OK) return rc;
     LG_ROWS(grad_out, grad_dtype, dim, grad_stride, n_ids, "grad_out");
     LG_ROWS(grad_table, table_dtype, dim, table_stride, n_nodes, "grad_table");
+    LG_ARG(n_ids == 0 || grad_table != grad_out, "grad_table must not be grad_out");
     const GradScratch w((uint8_t *)workspace, n_ids, dim);
     if (n_ids > 0 && (rc = check_workspace(workspace, workspace_bytes, w.bytes)) != LEGION_OK) return rc;
     const OnDevice on(dev_id);
@@ -1217,7 +1223,8 @@ extern "C" int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32
     LG_ROWS(grad_out, grad_dtype, dim, grad_stride, n_ids, "grad_out");
     LG_ROWS(grad_rows, LEGION_F32, dim, rows_stride, n_ids, "grad_rows");
     LG_ARG(count != nullptr && (uintptr_t)count % 4 == 0, "count is NULL");
-    LG_ARG(n_ids == 0 || (unique_ids != nullptr && (uintptr_t)unique_ids % id_bytes == 0), "unique_ids is NULL");
+    LG_ARG(n_ids == 0 || (unique_ids != nullptr && (uintptr_t)unique_ids % id_bytes == 0), "unique_ids is NULL or not on a multiple of the ids' width");
+    LG_ARG(n_ids == 0 || (unique_ids != ids && (const void *)grad_rows != grad_out), "unique_ids and grad_rows must not be the inputs");
     const GradScratch w((uint8_t *)workspace, n_ids, dim);
     if (n_ids > 0 && (rc = check_workspace(workspace, workspace_bytes, w.bytes)) != LEGION_OK) return rc;
     const OnDevice on(dev_id);

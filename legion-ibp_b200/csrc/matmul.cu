@@ -686,6 +686,7 @@ extern "C" int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *row
            "compressed rows are (feature_len + 4) rounded up to 16 bytes long, strides are multiples of 16 bytes");
     LG_ARG(dtype_known(out_dtype), "out: dtype must be LEGION_F32, LEGION_F16 or LEGION_BF16");
     LG_ARG(out_stride >= n && out_stride <= (1ll << 40) && (uintptr_t)out % dtype_bytes(out_dtype) == 0, "bad out stride or address");
+    LG_ARG(m == 0 || n == 0 || (out != rows && out != weight_rows), "out must not be one of the operands");
     if (m == 0 || n == 0) return LEGION_OK;
     const OnDevice on(dev_id);
     LG_CUDA(on.err);

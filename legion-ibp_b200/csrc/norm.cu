@@ -768,6 +768,8 @@ extern "C" int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int
         LG_ARG((uintptr_t)out % 16 == 0 && out_stride % 16 == 0 && out_stride >= code_row_bytes(dim),
                "compressed rows start on multiples of 16 bytes and are (dim + 4) rounded up to 16 bytes long");
     }
+    LG_ARG(n_rows == 0 || out != residual_out, "out and residual_out must be two buffers");
+    LG_ARG(n_rows == 0 || codec == LEGION_CODEC_RAW || (out != x && out != residual), "compressed rows cannot take the place of x or residual");
     if (n_rows == 0) return LEGION_OK;
     const OnDevice on(dev_id);
     LG_CUDA(on.err);
@@ -819,6 +821,7 @@ extern "C" int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_
     LG_OPERAND(grad_out, grad_stride, dim, dtype, "grad_out");
     LG_OPERAND(grad_x, grad_x_stride, dim, dtype, "grad_x");
     LG_OPERAND(grad_residual, grad_residual_stride, dim, dtype, "grad_residual");
+    LG_ARG(grad_weight != weight, "grad_weight must not be the weight");
     LG_ARG(n_rows == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace is NULL or not on a multiple of 16 bytes");
     LG_ARG(workspace_bytes >= norm_grad_scratch(n_rows, dim), "workspace is smaller than the call asks for");
     const OnDevice on(dev_id);

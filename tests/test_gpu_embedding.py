@@ -208,6 +208,48 @@ def test_gradient_nan_stays_in_its_row_and_strides():
     assert bool((rest == 7.0).all())
 
 
+@pytest.mark.parametrize("table_type,pad,shift", [("f32", 1, 1), ("f16", 3, 1), ("bf16", 2, 2), ("f32", 4, 0), ("f16", 8, 0)])
+@pytest.mark.parametrize("n,dim", [(5, 17), (700, 64), (3000, 130), (30000, 10)])
+def test_gradient_of_tables_with_strides(n, dim, table_type, pad, shift):
+    """Rows that no id names are zeroed, what lies between the rows is not."""
+    import torch
+    nodes = 900
+    ids = _ids(np.random.default_rng(n), n, nodes, False, 2.0)
+    grad = torch.randn(n, dim, device="cuda")
+    whole, out = _strided(nodes, dim, _types()[table_type], pad, shift)
+    L.embedding_grad(0, ids, grad, out, torch.empty(L.embedding_grad_workspace(n, dim, nodes), dtype=torch.uint8, device="cuda"), 0.25)
+    want, mag, count = _exact_grad(ids, grad, nodes, 0.25)
+    _close(out, want, mag * ((count[:, None] + 2).double() * U32))
+    rest = whole.clone()
+    torch.as_strided(rest, (nodes, dim), (dim + pad, 1), shift).fill_(7.0)
+    assert bool((rest == 7.0).all())
+
+
+def test_two_streams_at_once():
+    """Calls that share nothing but their inputs, on two streams, against the same calls one after the other."""
+    import torch
+    rng = np.random.default_rng(4)
+    nodes, dim = 4000, 256
+    table = torch.randn(nodes, dim, device="cuda").half()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    work = []
+    for n in (15000, 40000):
+        ids = _ids(rng, n, nodes, True, 3.0)
+        work.append((ids, torch.randn(n, dim, device="cuda"), [torch.empty(n, dim, device="cuda", dtype=torch.half) for _ in range(2)],
+                     [torch.empty(nodes, dim, device="cuda") for _ in range(2)],
+                     [torch.empty(L.embedding_grad_workspace(n, dim, nodes), dtype=torch.uint8, device="cuda") for _ in range(2)]))
+    torch.cuda.synchronize()
+    for turn in range(5):
+        for k, (ids, grad, out, whole, ws) in enumerate(work):
+            L.embedding_lookup(0, table, ids, out[0], 2.0, stream=sides[k])
+            L.embedding_grad(0, ids, grad, whole[0], ws[0], stream=sides[k])
+    torch.cuda.synchronize()
+    for ids, grad, out, whole, ws in work:
+        L.embedding_lookup(0, table, ids, out[1], 2.0)
+        L.embedding_grad(0, ids, grad, whole[1], ws[1])
+        assert torch.equal(out[0], out[1]) and torch.equal(whole[0], whole[1])
+
+
 def test_gradient_against_differences():
     """The lookup is linear in the table: <grad, step> is the difference of <out, weights> over any step."""
     import torch
@@ -227,10 +269,11 @@ def test_gradient_against_differences():
     assert abs(float((grad.double() * step.double()).sum() - difference)) <= slack
 
 
-def test_gradient_captured_and_replayed_on_another_stream():
+@pytest.mark.parametrize("n", [300, 9000, 50000])
+def test_gradient_captured_and_replayed_on_another_stream(n):
     """Two captured gradients with workspaces of their own, replayed over changed inputs, side by side with an eager one."""
     import torch
-    n, nodes, dim = 9000, 500, 64
+    nodes, dim = 500, 64
     rng = np.random.default_rng(11)
     sides = [torch.cuda.Stream() for _ in range(2)]
     made = []

@@ -174,6 +174,24 @@ def test_captured_with_other_rows():
         _check(out, c, b, 256, L.CODEC_INT8)
 
 
+def test_two_streams_at_once():
+    """Kernels that fill the chip, each with all of an SM's tensor memory, on two streams: the same as one after the other."""
+    import torch
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    work = [(_coded(m, k, L.CODEC_INT8, 0, 20 + m), _coded(n, k, L.CODEC_INT8, 0, 30 + n), k, torch.empty(m, n, device="cuda", dtype=torch.bfloat16))
+            for m, n, k in ((2000, 4000, 512), (300, 3000, 1024))]
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for k, (a, b, width, out) in enumerate(work):
+            L.matmul_rows(0, L.CODEC_INT8, a[0], b[0], width, out, stream=sides[k])
+    torch.cuda.synchronize()
+    for a, b, width, out in work:
+        again = torch.empty_like(out)
+        L.matmul_rows(0, L.CODEC_INT8, a[0], b[0], width, again)
+        assert torch.equal(out, again)
+    assert L.operator_error(0) == 0
+
+
 def test_nothing_to_do_and_refusals():
     import torch
     a, b = _coded(4, 64, 1)[0], _coded(6, 64, 1)[0]

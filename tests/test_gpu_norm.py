@@ -172,12 +172,13 @@ def test_rows_of_zeros_infinities_and_large_values():
     _close(out[keep], want[keep], want[keep].abs() * (32 * U32))
 
 
-def test_captured_on_another_stream():
+@pytest.mark.parametrize("n,dim", [(300, 512), (1300, 2048)])
+def test_captured_on_another_stream(n, dim):
     import torch
-    x, w, r = _inputs(300, 512, torch.bfloat16, torch.float32, True)
+    x, w, r = _inputs(n, dim, torch.bfloat16, torch.float32, True)
     out, total = torch.empty_like(x), torch.empty_like(x)
     dx, dw = torch.empty_like(x), torch.empty_like(w)
-    ws = torch.empty(L.rms_norm_grad_workspace(300, 512), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda")
     side = torch.cuda.Stream()
     L.rms_norm(0, x, w, out, 1e-6, r, total)
     L.rms_norm_grad(0, out, total, w, dx, dw, ws, 1e-6, r)
@@ -188,7 +189,7 @@ def test_captured_on_another_stream():
         L.rms_norm(0, x, w, out, 1e-6, r, total, stream=s)
         L.rms_norm_grad(0, out, total, w, dx, dw, ws, 1e-6, r, stream=s)
     for _ in range(2):
-        x.copy_(torch.randn(300, 512, device="cuda"))
+        x.copy_(torch.randn(n, dim, device="cuda"))
         torch.cuda.synchronize()
         with torch.cuda.stream(side):
             graph.replay()

@@ -46,6 +46,8 @@ BAD = [
     ("norm", dict(codec=1, dim=6, out_stride=16)), ("norm_grad", dict(ws_bytes=31, n_rows=1)), ("norm_grad", dict(ws=None, n_rows=1)),
     ("matmul", dict(codec=3)), ("matmul", dict(k=0)), ("matmul", dict(k=6)), ("matmul", dict(row_stride=24)), ("matmul", dict(row_stride=0)),
     ("matmul", dict(k=16)), ("matmul", dict(m=-1)), ("matmul", dict(n=-1)), ("matmul", dict(table=A + 4)), ("matmul", dict(weight=A + 8)),
+    ("lookup grad rows", dict(n_ids=1)), ("norm", dict(n_rows=1, codec=2, out_stride=16)), ("norm_grad", dict(n_rows=1)), ("matmul", dict(m=1, n=1)),   # outputs that are inputs
+    ("lookup", dict(n_ids=1 << 28, dim=1 << 16, stride=1 << 16, table_stride=1 << 16, out_stride=1 << 16, out=2 * A)),
     ("matmul", dict(n=9, m=1)), ("matmul", dict(m=1, n=1, table=None)), ("matmul", dict(k=131072, row_stride=1 << 18)),
 ]
 
