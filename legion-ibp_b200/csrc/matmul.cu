@@ -270,6 +270,9 @@ __device__ __forceinline__ void store_turned(uint32_t acc, float ps, const float
 // The output leaves by TMA: a warp writes 128 bytes of each of its 32 rows to shared memory (in the swizzle that the store
 // undoes, so that lanes hit different banks); rows that TMA cannot address are written by the lanes along the rows (every lane along its
 // own row, 510 x 7548 bf16 took 47 us).
+// What bounds it: large products of rows on 128-byte boundaries the tensor cores (4096 x 16384 x 4096 int8: 171 us, 3.2 POP/s); rows that
+// start on 16-byte boundaries, as compressed rows do, the copy engine, which takes 278 clocks for 128 of them where the products of
+// a stage take 512 (214 us; 128 x 256 tiles of one CTA: 342 us); few rows the weights' bytes (16 rows: 18 us for 67 MB).
 // P_OUT_COLUMNS: rows of P are columns of the output (P holds the weights), for few rows on the other side.  A tile then has step_p rows of P,
 // as many as spread the weights over all SMs.  The products read 128 rows all the same: what lies behind the tile's rows in shared
 // memory reaches nobody's sums but those of rows that are not stored.
