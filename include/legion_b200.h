@@ -425,6 +425,52 @@ int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t 
  * inside legion_matmul_rows or legion_rms_norm_grad did not complete within its wait limit, the call's output is not valid).  Waits for `stream`. */
 int legion_operator_error(int32_t dev_id, void *stream, int32_t *error, int32_t reset);
 
+/* The operators above with their arguments in one block, for bindings that pay per argument (a ctypes call costs 0.1 us for each).  A block
+ * begins with the operator's number and its own size in bytes; its fields are the call's arguments, 8-byte ones first, without padding. */
+#define LEGION_OP_EMBEDDING_LOOKUP 1
+#define LEGION_OP_EMBEDDING_GRAD 2
+#define LEGION_OP_EMBEDDING_GRAD_ROWS 3
+#define LEGION_OP_RMS_NORM 4
+#define LEGION_OP_RMS_NORM_GRAD 5
+#define LEGION_OP_MATMUL_ROWS 6
+typedef struct LegionCallHead { int32_t op, bytes; } LegionCallHead;
+typedef struct LegionEmbeddingLookupArgs {
+    LegionCallHead head;
+    const void *table; int64_t table_stride, n_nodes; const void *ids; int64_t n_ids; void *out; int64_t out_stride; void *stream;
+    int32_t dev_id, table_dtype, id_bytes, dim, out_dtype; float scale;
+} LegionEmbeddingLookupArgs;
+typedef struct LegionEmbeddingGradArgs {
+    LegionCallHead head;
+    const void *ids; int64_t n_ids; const void *grad_out; int64_t grad_stride; void *grad_table; int64_t table_stride, n_nodes;
+    void *workspace; int64_t workspace_bytes; void *stream;
+    int32_t dev_id, id_bytes, grad_dtype, dim, table_dtype, accumulate; float scale; int32_t unused;
+} LegionEmbeddingGradArgs;
+typedef struct LegionEmbeddingGradRowsArgs {
+    LegionCallHead head;
+    const void *ids; int64_t n_ids; const void *grad_out; int64_t grad_stride, n_nodes; void *unique_ids; float *grad_rows;
+    int64_t rows_stride; int32_t *count; void *workspace; int64_t workspace_bytes; void *stream;
+    int32_t dev_id, id_bytes, grad_dtype, dim; float scale; int32_t unused;
+} LegionEmbeddingGradRowsArgs;
+typedef struct LegionRmsNormArgs {
+    LegionCallHead head;
+    const void *x; int64_t x_stride; const void *residual; int64_t residual_stride; const void *weight; int64_t n_rows; void *out;
+    int64_t out_stride; void *residual_out; int64_t residual_out_stride; void *stream;
+    int32_t dev_id, dtype, weight_dtype, dim, codec; float eps;
+} LegionRmsNormArgs;
+typedef struct LegionRmsNormGradArgs {
+    LegionCallHead head;
+    const void *grad_out; int64_t grad_stride; const void *x; int64_t x_stride; const void *grad_residual; int64_t grad_residual_stride;
+    const void *weight; int64_t n_rows; void *grad_x; int64_t grad_x_stride; void *grad_weight; void *workspace; int64_t workspace_bytes;
+    void *stream;
+    int32_t dev_id, dtype, weight_dtype, dim, grad_weight_dtype; float eps;
+} LegionRmsNormGradArgs;
+typedef struct LegionMatmulRowsArgs {
+    LegionCallHead head;
+    const void *rows; int64_t m, row_stride; const void *weight_rows; int64_t n, weight_stride; void *out; int64_t out_stride; void *stream;
+    int32_t dev_id, codec, feature_len, out_dtype;
+} LegionMatmulRowsArgs;
+int legion_operator_call(const void *block);
+
 /* ---- whole batch --------------------------------------------------------------------- */
 
 /* The op list of GPURunner::RunOnce (engine/server.cu:342-351) for one batch on one stream set.

@@ -545,3 +545,63 @@ extern "C" int legion_enable_peer_access(int32_t dev_id, int32_t peer_id)
     LG_CUDA(e);
     return LEGION_OK;
 }
+
+// ---- operators on learned and compressed rows, arguments in one block ----------------------------------------------------
+
+template <typename A>
+static int block_of(const void *block, int32_t bytes, A *args)
+{
+    LG_ARG(bytes == (int32_t)sizeof(A), "the block's size is not that of the operator's arguments");
+    memcpy(args, block, sizeof(A));
+    return LEGION_OK;
+}
+
+extern "C" int legion_operator_call(const void *block)
+{
+    LG_ARG(block != nullptr, "block is NULL");
+    LegionCallHead head;
+    memcpy(&head, block, sizeof(head));
+    int rc;
+    switch (head.op) {
+    case LEGION_OP_EMBEDDING_LOOKUP: {
+        LegionEmbeddingLookupArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_embedding_lookup(a.dev_id, a.table, a.table_dtype, a.table_stride, a.n_nodes, a.ids, a.id_bytes, a.n_ids, a.dim, a.scale,
+                                       a.out, a.out_dtype, a.out_stride, a.stream);
+    }
+    case LEGION_OP_EMBEDDING_GRAD: {
+        LegionEmbeddingGradArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_embedding_grad(a.dev_id, a.ids, a.id_bytes, a.n_ids, a.grad_out, a.grad_dtype, a.grad_stride, a.dim, a.scale, a.grad_table,
+                                     a.table_dtype, a.table_stride, a.n_nodes, a.accumulate, a.workspace, a.workspace_bytes, a.stream);
+    }
+    case LEGION_OP_EMBEDDING_GRAD_ROWS: {
+        LegionEmbeddingGradRowsArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_embedding_grad_rows(a.dev_id, a.ids, a.id_bytes, a.n_ids, a.grad_out, a.grad_dtype, a.grad_stride, a.dim, a.scale, a.n_nodes,
+                                          a.unique_ids, a.grad_rows, a.rows_stride, a.count, a.workspace, a.workspace_bytes, a.stream);
+    }
+    case LEGION_OP_RMS_NORM: {
+        LegionRmsNormArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_rms_norm(a.dev_id, a.x, a.dtype, a.x_stride, a.residual, a.residual_stride, a.weight, a.weight_dtype, a.eps, a.n_rows, a.dim,
+                               a.codec, a.out, a.out_stride, a.residual_out, a.residual_out_stride, a.stream);
+    }
+    case LEGION_OP_RMS_NORM_GRAD: {
+        LegionRmsNormGradArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_rms_norm_grad(a.dev_id, a.grad_out, a.grad_stride, a.x, a.x_stride, a.dtype, a.grad_residual, a.grad_residual_stride, a.weight,
+                                    a.weight_dtype, a.eps, a.n_rows, a.dim, a.grad_x, a.grad_x_stride, a.grad_weight, a.grad_weight_dtype,
+                                    a.workspace, a.workspace_bytes, a.stream);
+    }
+    case LEGION_OP_MATMUL_ROWS: {
+        LegionMatmulRowsArgs a;
+        if ((rc = block_of(block, head.bytes, &a)) != LEGION_OK) return rc;
+        return legion_matmul_rows(a.dev_id, a.codec, a.rows, a.m, a.row_stride, a.weight_rows, a.n, a.weight_stride, a.feature_len, a.out,
+                                  a.out_dtype, a.out_stride, a.stream);
+    }
+    default: break;
+    }
+    set_error("legion_operator_call: unknown operator %d", head.op);
+    return LEGION_E_ARG;
+}

@@ -60,6 +60,17 @@ def test_bad_arguments_are_refused(names, change):
         assert L.lib().legion_last_error()
 
 
+def test_blocks_have_the_size_of_the_structs():
+    """A block of another size, or of no operator, is refused; one of the right size reaches the operator's own checks."""
+    call, error = L.lib().legion_operator_call, L.lib().legion_last_error
+    for op, s in ((1, L._LOOKUP), (2, L._GRAD), (3, L._GRAD_ROWS), (4, L._NORM), (5, L._NORM_GRAD), (6, L._MATMUL)):
+        empty = lambda size: op.to_bytes(4, "little") + size.to_bytes(4, "little") + bytes(s.size - 8)
+        assert call(empty(s.size + 8)) == -1 and b"size" in error()
+        assert call(empty(s.size)) == -1 and b"block" not in error()
+    assert call((99).to_bytes(4, "little") + bytes(100)) == -1 and b"unknown" in error()
+    assert call(None) == -1
+
+
 def test_nothing_to_do_is_no_error_without_a_gpu():
     for name in ("lookup", "norm", "matmul"):
         assert _calls()[name]() == 0
