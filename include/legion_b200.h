@@ -397,7 +397,7 @@ int legion_embedding_grad_rows(int32_t dev_id, const void *ids, int32_t id_bytes
 /* h = x + residual (residual may be NULL), out = h * weight / sqrt(mean(h^2) + eps) over rows of dim elements.  x, residual,
  * residual_out (h rounded once; may be NULL) and, codec RAW, out are of `dtype`; weight is fp32 or of that type.  codec INT8 or E4M3:
  * out receives compressed rows, out_stride bytes apart (a multiple of 16): dim codes, an fp32 scale, zeros up to a multiple of 16
- * bytes, exactly what legion_quantize_table makes of the fp32 rows (dim % 4 == 0).  out and residual_out may be x or residual
+ * bytes, exactly what legion_quantize_table makes of the fp32 rows (dim % 4 == 0).  residual_out and, codec RAW, out may be x or residual
  * themselves (same address and stride), but not each other; other overlaps are not allowed.  h and its squares are fp32: a
  * row whose squares sum to more than 3.4e38 has an infinite mean.  With eps 0 a row of zeros has no finite norm: its result is NaN. */
 int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stride, const void *residual,
@@ -406,8 +406,8 @@ int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stri
 int legion_rms_norm_grad_workspace(int64_t n_rows, int32_t dim, int64_t *bytes);
 /* The norm's gradient.  x: the rows that were normed (with a residual: residual_out).  grad_x = the gradient of x by way of out, plus
  * grad_residual (the gradient that reached residual_out otherwise; may be NULL); with a residual it is the gradient
- * of both.  grad_weight (dim elements, fp32 or the rows' type) is set, not added to.  grad_x may be grad_out, x or grad_residual.
- * Workspace as above. */
+ * of both.  grad_weight (dim elements, fp32 or the rows' type) is set, not added to.  grad_x may be grad_out, x or grad_residual (same address and
+ * stride).  Workspace as above. */
 int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_t grad_stride, const void *x, int64_t x_stride,
                          int32_t dtype, const void *grad_residual, int64_t grad_residual_stride, const void *weight,
                          int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim, void *grad_x, int64_t grad_x_stride,

@@ -746,6 +746,9 @@ using namespace legion;
     LG_ARG((uintptr_t)(p) % dtype_bytes(dtype) == 0, what " must start on a multiple of its element's size"); \
     LG_ARG((p) == nullptr || ((stride) >= (dim) && (stride) <= (1ll << 40)), what ": a row's stride must be at least its length")
 
+// Rows in the place of other rows: one by one, or each would be written over others that are not read yet.
+static bool same_stride(const void *a, int64_t a_stride, const void *b, int64_t b_stride) { return a == nullptr || a != b || a_stride == b_stride; }
+
 extern "C" int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stride, const void *residual,
                                int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim,
                                int32_t codec, void *out, int64_t out_stride, void *residual_out, int64_t residual_out_stride, void *stream)
@@ -770,6 +773,10 @@ extern "C" int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int
     }
     LG_ARG(n_rows == 0 || out != residual_out, "out and residual_out must be two buffers");
     LG_ARG(n_rows == 0 || codec == LEGION_CODEC_RAW || (out != x && out != residual), "compressed rows cannot take the place of x or residual");
+    LG_ARG(n_rows <= 1 || (same_stride(out, out_stride, x, x_stride) && same_stride(out, out_stride, residual, residual_stride) &&
+                           same_stride(residual_out, residual_out_stride, x, x_stride) &&
+                           same_stride(residual_out, residual_out_stride, residual, residual_stride)),
+           "an output in an input's place must have its stride");
     if (n_rows == 0) return LEGION_OK;
     const OnDevice on(dev_id);
     LG_CUDA(on.err);
@@ -821,6 +828,9 @@ extern "C" int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_
     LG_OPERAND(grad_out, grad_stride, dim, dtype, "grad_out");
     LG_OPERAND(grad_x, grad_x_stride, dim, dtype, "grad_x");
     LG_OPERAND(grad_residual, grad_residual_stride, dim, dtype, "grad_residual");
+    LG_ARG(n_rows <= 1 || (same_stride(grad_x, grad_x_stride, grad_out, grad_stride) && same_stride(grad_x, grad_x_stride, x, x_stride) &&
+                           same_stride(grad_x, grad_x_stride, grad_residual, grad_residual_stride)),
+           "grad_x in an input's place must have its stride");
     LG_ARG(grad_weight != weight, "grad_weight must not be the weight");
     LG_ARG(n_rows == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "workspace is NULL or not on a multiple of 16 bytes");
     LG_ARG(workspace_bytes >= norm_grad_scratch(n_rows, dim), "workspace is smaller than the call asks for");

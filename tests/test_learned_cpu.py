@@ -60,6 +60,21 @@ def test_bad_arguments_are_refused(names, change):
         assert L.lib().legion_last_error()
 
 
+@pytest.mark.parametrize("output", ["out", "residual_out", "grad_x"])
+@pytest.mark.parametrize("input", [0, 1, 2])
+def test_rows_in_place_keep_their_stride(output, input):
+    """An output in an input's place but with other distances between its rows would be written over rows not read yet."""
+    l, at, n = L.lib(), (A, 2 * A, 3 * A), 2
+    if output == "grad_x":
+        rc = l.legion_rms_norm_grad(0, at[0], 8, at[1], 8, L.F32, at[2], 8, 9 * A, L.F32, 1e-6, n, 8, at[input], 16, 5 * A, L.F32, 6 * A, 1 << 20, None)
+    elif input == 2:
+        return
+    else:
+        out, other = (at[input], 7 * A) if output == "out" else (7 * A, at[input])
+        rc = l.legion_rms_norm(0, at[0], L.F32, 8, at[1], 8, 9 * A, L.F32, 1e-6, n, 8, 0, out, 16, other, 16, None)
+    assert rc == -1 and b"stride" in l.legion_last_error()
+
+
 def test_blocks_have_the_size_of_the_structs():
     """A block of another size, or of no operator, is refused; one of the right size reaches the operator's own checks."""
     call, error = L.lib().legion_operator_call, L.lib().legion_last_error
