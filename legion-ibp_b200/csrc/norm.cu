@@ -22,6 +22,39 @@ __device__ int32_t g_norm_error = 0;
 __device__ __forceinline__ void raise_operator_error() { atomicCAS(&g_norm_error, 0, LEGION_E_TIMEOUT); }
 cudaError_t norm_error_word(void **word) { return cudaGetSymbolAddress(word, g_norm_error); }
 
+// Two fp32 values that one instruction works on, each rounded as it would be alone.
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ static Two of(float a, float b)
+    {
+        Two t;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(a), "f"(b));
+        return t;
+    }
+    __device__ __forceinline__ float low() const { return __uint_as_float((uint32_t)v); }
+    __device__ __forceinline__ float high() const { return __uint_as_float((uint32_t)(v >> 32)); }
+    __device__ __forceinline__ float sum() const { return low() + high(); }
+};
+__device__ __forceinline__ Two operator*(const Two &a, const Two &b)
+{
+    Two t;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+    return t;
+}
+__device__ __forceinline__ Two fma(const Two &a, const Two &b, const Two &c)
+{
+    Two t;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return t;
+}
+// 1 / sqrt(x): rsqrtf's value, off by up to two units in the last place, after one of Newton's steps, which leaves the roundings of x r and
+// of the result; at 0 and infinity as rsqrtf has it.
+__device__ __forceinline__ float inverse_root(float x)
+{
+    const float r = rsqrtf(x);
+    return r > 0.0f && r < INFINITY ? fmaf(0.5f * r, fmaf(-x * r, r, 1.0f), r) : r;
+}
+
 // Sum and, WITH_MAX, NaN-keeping maximum over the threads of a row.  GROUP lanes of a warp, or (0) the CTA.
 template <int GROUP>
 struct RowReduce {
@@ -338,17 +371,24 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
             }
         }
     };
-    // wider threads have no registers for it (12371 rows of 602 fp32: 51 us with it, 32 without)
+    // wider threads have no registers for it (12371 rows of 602 fp32: 51 us with it, 32 without, 28 since two elements share an instruction)
     constexpr bool kAhead = U * VE * (int)sizeof(T) <= 64 && MAXT <= 256;
     const int64_t step = (int64_t)gridDim.x * per_cta;
     if (kAhead) fetch((int64_t)blockIdx.x * per_cta + mate);
-    float w[U][VE], dw[U][VE];
+    // the thread's elements in pairs, whatever vectors they came by (a thread of one element has half a pair)
+    constexpr int E = U * VE, P = (E + 1) / 2;
+    float x[2 * P];
+    x[2 * P - 1] = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, w[u]);
+    for (int u = 0; u < U; ++u) load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, x + u * VE);
+    Two w[P], dw[P];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) dw[u][i] = 0.0f;
+    for (int j = 0; j < P; ++j) {
+        w[j] = Two::of(x[2 * j], x[2 * j + 1]);
+        dw[j] = Two::of(0.0f, 0.0f);
     }
+    auto pair = [&](const Vec<T, VE> *v, int j) { return Two::of(v[2 * j / VE].get(2 * j % VE), 2 * j + 1 < E ? v[(2 * j + 1) % E / VE].get((2 * j + 1) % VE) : 0.0f); };
+    const float per_dim = 1.0f / (float)p.dim;
     for (int64_t row0 = (int64_t)blockIdx.x * per_cta; row0 < p.n; row0 += step) {
         const int64_t row = row0 + mate;
         const bool in = row < p.n;
@@ -361,34 +401,40 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
             r[u] = next_r[u];
         }
         if (kAhead && row0 + step < p.n) fetch(row + step);  // the next row is on its way while this one is worked on
-        float square = 0.0f, dot = 0.0f;
+        Two square2 = Two::of(0.0f, 0.0f), dot2 = square2;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float a = h[u].get(i);
-                square = fmaf(a, a, square);
-                dot = fmaf(dy[u].get(i) * w[u][i], a, dot);
-            }
+        for (int j = 0; j < P; ++j) {
+            const Two a = pair(h, j);
+            square2 = fma(a, a, square2);
+            dot2 = fma(pair(dy, j) * w[j], a, dot2);
+        }
+        float square = square2.sum(), dot = dot2.sum();
         reduce.two(square, dot, false);
-        const float s = 1.0f / sqrtf(square / (float)p.dim + p.eps);
-        const float k = s * s * s * (dot / (float)p.dim);
+        const float s = inverse_root(fmaf(square, per_dim, p.eps));
+        const float k = s * s * s * (dot * per_dim);
+        const Two s2 = Two::of(s, s), k2 = Two::of(-k, -k);
+        float dx[2 * P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const Two a = pair(h, j), g = pair(dy, j);
+            const Two d = fma(a, k2, fma(g * w[j], s2, pair(r, j)));
+            dx[2 * j] = d.low();
+            dx[2 * j + 1] = d.high();
+            if (in) dw[j] = fma(g, a * s2, dw[j]);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int col = (t + u * width) * VE;
             if (!in || col >= p.dim) continue;
-            float dx[VE];
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float a = h[u].get(i), g = dy[u].get(i);
-                dx[i] = s * (g * w[u][i]) - a * k;
-                if (p.grad_residual != nullptr) dx[i] += r[u].get(i);
-                dw[u][i] = fmaf(g, a * s, dw[u][i]);
-            }
             Vec<T, VE> o;
-            o.set(dx);
+            o.set(dx + u * VE);
             o.store(static_cast<T *>(p.grad_x) + row * p.grad_x_stride + col);
         }
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        x[2 * j] = dw[j].low();
+        x[2 * j + 1] = dw[j].high();
     }
     float *part = p.part + (int64_t)blockIdx.x * p.dim;
     if (GROUP == 0) {
@@ -396,7 +442,7 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < VE; ++i)
-                if ((t + u * width) * VE < p.dim) part[(t + u * width) * VE + i] = dw[u][i];
+                if ((t + u * width) * VE < p.dim) part[(t + u * width) * VE + i] = x[u * VE + i];
         return;
     }
     // the groups of a CTA add theirs in group order
@@ -404,7 +450,7 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) cross[(threadIdx.x / (GROUP == 0 ? 1 : GROUP)) * kCols + (t + u * GROUP) * VE + i] = dw[u][i];
+        for (int i = 0; i < VE; ++i) cross[(threadIdx.x / (GROUP == 0 ? 1 : GROUP)) * kCols + (t + u * GROUP) * VE + i] = x[u * VE + i];
     __syncthreads();
     for (int col = threadIdx.x; col < p.dim; col += 128) {
         float sum = 0.0f;
@@ -413,18 +459,57 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
     }
 }
 
+// Sums of N values each over the threads of a CTA, for N of 2 or 4 and at most 32 / N warps: halves of the lanes take over half of the values as
+// the lanes are added up, so that N values cost little more than one.  One barrier.
+template <int N>
+__device__ __forceinline__ void sums_of_cta(float *v, float *smem, int &flip)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int d = 16;
+#pragma unroll
+    for (int n = N; n > 1; n /= 2, d /= 2) {
+        const bool upper = lane & d;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float give = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+            v[i] = keep + __shfl_xor_sync(kFull, give, d);
+        }
+    }
+#pragma unroll
+    for (; d > 0; d /= 2) v[0] += __shfl_xor_sync(kFull, v[0], d);
+    // the lane's value: the bits of the lane from the highest on
+    constexpr int kLanes = 32 / N;
+    float *s = smem + flip * 32;
+    flip ^= 1;
+    const int warps = blockDim.x >> 5;
+    if (lane % kLanes == 0) s[lane + warp] = v[0];
+    __syncthreads();
+    float x = lane % kLanes < warps ? s[lane] : 0.0f;
+#pragma unroll
+    for (int e = kLanes / 2; e > 0; e /= 2) x += __shfl_xor_sync(kFull, x, e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kFull, x, i * kLanes);
+}
+
 // The same for long rows on 16-byte boundaries, where there are many: one thread has the copy engine bring whole rows into shared memory,
 // `stages` rows ahead, so that what is on its way does not depend on registers.  A stage is free again when the threads
-// have met in the row's reduction: by then all of them have read their part of it.
-// Measured, 16384 rows of 2048 bf16 (268 MB): 64 us with the next row in registers, 72 without it.
-template <typename T, int U, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_grad_stream_kernel(NormGradParams p, int stages)
+// have met in the row's reduction: by then all of them have read their part of it.  R rows meet in one reduction (stages: a multiple of R):
+// what bounds a CTA is that meeting, and the instructions (hence pairs of fp32).
+// Measured, 16384 rows of 2048 bf16 with residual (268 MB): 49 us a call, 5.5 TB/s; one row a meeting 53.5; single fp32 and the reduction of one row at a
+// time 60; the next row in registers 64, without it 72.
+template <typename T, int U, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) norm_grad_stream_kernel(NormGradParams p, int stages)
 {
     constexpr int VE = 16 / (int)sizeof(T);
+    // a CTA of many threads has no registers for a row and reads it from its stage again, which is free a row later then (with the row in
+    // spilled registers, 4000 rows of 12000 bf16 took 360 us, like this 61)
+    constexpr bool kAgain = MAXT > 256;
+    static_assert(R == 1 || !kAgain, "the stage before is one row's");
     extern __shared__ __align__(128) uint8_t rows[];   // [stage][x, grad_out, grad_residual][row]
     __shared__ float smem[128];
     __shared__ uint64_t bars[kStreamStages];
     RowReduce<0> reduce(smem);
+    int flip = 0;
     const int t = threadIdx.x, width = blockDim.x;
     const uint32_t row_bytes = (uint32_t)p.dim * sizeof(T);
     const int arrays = p.grad_residual != nullptr ? 3 : 2;
@@ -443,61 +528,95 @@ __global__ void __launch_bounds__(MAXT) norm_grad_stream_kernel(NormGradParams p
         for (int s = 0; s < stages; ++s)
             if (blockIdx.x + s * step < p.n) bring(blockIdx.x + s * step, s);
     }
-    float w[U][VE], dw[U][VE];
+    Two w[U][VE / 2], dw[U][VE / 2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, w[u]);
+        float x[VE];
+        load_weight<T, VE>(p.weight, p.weight_dtype, (t + u * width) * VE, p.dim, x);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) dw[u][i] = 0.0f;
+        for (int i = 0; i < VE / 2; ++i) {
+            w[u][i] = Two::of(x[2 * i], x[2 * i + 1]);
+            dw[u][i] = Two::of(0.0f, 0.0f);
+        }
     }
+    const float per_dim = 1.0f / (float)p.dim;
     __syncthreads();
     int stage = 0;
     uint32_t phase = 0, tries = kWaitTries;
-    for (int64_t row = blockIdx.x; row < p.n; row += step) {
-        if (!wait_barrier(shared_addr(&bars[stage]), phase, tries)) tries = 0;   // given up: the rest is not waited for, the error is kept
-        const uint8_t *src = rows + (size_t)stage * arrays * row_bytes;
-        Vec<T, VE> h[U], dy[U], r[U];
-        float square = 0.0f, dot = 0.0f;
+    for (int64_t row = blockIdx.x; row < p.n; row += R * step) {
+        Vec<T, VE> h[R][U], dy[R][U], r[R][U];
+        const uint8_t *src[R];
+        float sums[2 * R];   // of the rows' squares, then of dy w h
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int col = (t + u * width) * VE;
-            h[u].zero();
-            dy[u].zero();
-            r[u].zero();
-            if (col < p.dim) {
-                h[u].load(reinterpret_cast<const T *>(src) + col);
-                dy[u].load(reinterpret_cast<const T *>(src + row_bytes) + col);
-                if (arrays == 3) r[u].load(reinterpret_cast<const T *>(src + 2 * row_bytes) + col);
+        for (int q = 0; q < R; ++q) {
+            const bool in = row + q * step < p.n;
+            if (in && !wait_barrier(shared_addr(&bars[stage + q]), phase, tries)) tries = 0;   // given up: the rest is not waited for, the error is kept
+            src[q] = rows + (size_t)(stage + q) * arrays * row_bytes;
+            Two square = Two::of(0.0f, 0.0f), dot = square;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int col = (t + u * width) * VE;
+                h[q][u].zero();
+                dy[q][u].zero();
+                r[q][u].zero();
+                if (in && col < p.dim) {
+                    h[q][u].load(reinterpret_cast<const T *>(src[q]) + col);
+                    dy[q][u].load(reinterpret_cast<const T *>(src[q] + row_bytes) + col);
+                    if (!kAgain && arrays == 3) r[q][u].load(reinterpret_cast<const T *>(src[q] + 2 * row_bytes) + col);
+                }
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    const Two a = Two::of(h[q][u].get(2 * i), h[q][u].get(2 * i + 1));
+                    square = fma(a, a, square);
+                    dot = fma(Two::of(dy[q][u].get(2 * i), dy[q][u].get(2 * i + 1)) * w[u][i], a, dot);
+                }
             }
+            sums[q] = square.sum();
+            sums[R + q] = dot.sum();
+        }
+        if (MAXT <= 256) sums_of_cta<2 * R>(sums, smem, flip);
+        else reduce.two(sums[0], sums[R], false);
+        if (t == 0 && tries != 0) {
+            if (kAgain) {   // the row before is done with
+                if (row >= step && row + (stages - 1) * step < p.n) bring(row + (stages - 1) * step, stage == 0 ? stages - 1 : stage - 1);
+            } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float a = h[u].get(i);
-                square = fmaf(a, a, square);
-                dot = fmaf(dy[u].get(i) * w[u][i], a, dot);
+                for (int q = 0; q < R; ++q)
+                    if (row + (stages + q) * step < p.n) bring(row + (stages + q) * step, stage + q);
             }
         }
-        reduce.two(square, dot, false);
-        if (t == 0 && row + stages * step < p.n && tries != 0) bring(row + stages * step, stage);
-        if (++stage == stages) {
+        stage += R;
+        if (stage == stages) {
             stage = 0;
             phase ^= 1;
         }
-        const float s = 1.0f / sqrtf(square / (float)p.dim + p.eps);
-        const float k = s * s * s * (dot / (float)p.dim);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int col = (t + u * width) * VE;
-            if (col >= p.dim) continue;
-            float dx[VE];
+        for (int q = 0; q < R; ++q) {
+            const float s = inverse_root(fmaf(sums[q], per_dim, p.eps));
+            const float k = s * s * s * (sums[R + q] * per_dim);
+            const Two s2 = Two::of(s, s), k2 = Two::of(-k, -k);
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float a = h[u].get(i), g = dy[u].get(i);
-                dx[i] = s * (g * w[u][i]) - a * k + r[u].get(i);
-                dw[u][i] = fmaf(g, a * s, dw[u][i]);
+            for (int u = 0; u < U; ++u) {
+                const int col = (t + u * width) * VE;
+                if (col >= p.dim || row + q * step >= p.n) continue;
+                if (kAgain) {
+                    h[q][u].load(reinterpret_cast<const T *>(src[q]) + col);
+                    dy[q][u].load(reinterpret_cast<const T *>(src[q] + row_bytes) + col);
+                    if (arrays == 3) r[q][u].load(reinterpret_cast<const T *>(src[q] + 2 * row_bytes) + col);
+                }
+                float dx[VE];
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    const Two a = Two::of(h[q][u].get(2 * i), h[q][u].get(2 * i + 1)), g = Two::of(dy[q][u].get(2 * i), dy[q][u].get(2 * i + 1));
+                    const Two d = fma(a, k2, fma(g * w[u][i], s2, Two::of(r[q][u].get(2 * i), r[q][u].get(2 * i + 1))));
+                    dx[2 * i] = d.low();
+                    dx[2 * i + 1] = d.high();
+                    dw[u][i] = fma(g, a * s2, dw[u][i]);
+                }
+                Vec<T, VE> o;
+                o.set(dx);
+                o.store(static_cast<T *>(p.grad_x) + (row + q * step) * p.grad_x_stride + col);
             }
-            Vec<T, VE> o;
-            o.set(dx);
-            o.store(static_cast<T *>(p.grad_x) + row * p.grad_x_stride + col);
         }
     }
     float *part = p.part + (int64_t)blockIdx.x * p.dim;
@@ -505,8 +624,14 @@ __global__ void __launch_bounds__(MAXT) norm_grad_stream_kernel(NormGradParams p
     for (int u = 0; u < U; ++u) {
         const int col = (t + u * width) * VE;
         if (col >= p.dim) continue;
+        float x[VE];
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+            x[2 * i] = dw[u][i].low();
+            x[2 * i + 1] = dw[u][i].high();
+        }
         Vec<float, VE> o;
-        o.set(dw[u]);
+        o.set(x);
         o.store(part + col);
     }
     if (tries == 0) {
@@ -657,10 +782,10 @@ static int launch_norm_codec(cudaStream_t s, const NormParams &p, int codec, int
     return launch_norm_ve<T, LEGION_CODEC_E4M3>(s, p, ve);
 }
 
-template <typename T, int U, int MAXT>
+template <typename T, int U, int R, int MAXT>
 static int launch_norm_grad_stream(cudaStream_t s, const NormGradParams &p, int threads, int *parts)
 {
-    const void *kernel = (const void *)norm_grad_stream_kernel<T, U, MAXT>;
+    const void *kernel = (const void *)norm_grad_stream_kernel<T, U, R, MAXT>;
     static bool allowed[64];
     const int rc = allow_smem(kernel, kStreamSmem, allowed);
     if (rc != LEGION_OK) return rc;
@@ -669,12 +794,13 @@ static int launch_norm_grad_stream(cudaStream_t s, const NormGradParams &p, int 
     int fit = 0;
     LG_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, 0));
     if (fit > kGradCtas / kSms) fit = kGradCtas / kSms;
-    while (fit > 1 && kStreamSmem / fit < 2 * stage) --fit;
+    while (fit > 1 && kStreamSmem / fit < 2 * R * stage) --fit;
     int stages = kStreamSmem / (fit < 1 ? 1 : fit) / stage;
     if (stages > kStreamStages) stages = kStreamStages;
+    stages -= stages % R;
     const int64_t most = (int64_t)(fit < 1 ? 1 : fit) * kSms;
     *parts = (int)(p.n < most ? p.n : most);
-    norm_grad_stream_kernel<T, U, MAXT><<<*parts, threads, stages * stage, s>>>(p, stages);
+    norm_grad_stream_kernel<T, U, R, MAXT><<<*parts, threads, stages * stage, s>>>(p, stages);
     LG_LAUNCH_CHECK();
     return LEGION_OK;
 }
@@ -685,17 +811,19 @@ static int launch_norm_grad(cudaStream_t s, const NormGradParams &p, int *parts)
     if constexpr (VE * sizeof(T) == 16) {
         const int64_t bytes = (int64_t)p.dim * sizeof(T), stage = (p.grad_residual != nullptr ? 3 : 2) * bytes;
         const int vecs = p.dim / VE;
-        // (20000 rows of 2048 bytes: 47 us like this, 34 by a warp each; 16384 of 4096: 61 and 64; 4000 of 16 KB: 58 and 88)
-        if (bytes >= 4096 && p.n >= 4 * kSms && 2 * stage <= kStreamSmem) {
+        // (20000 rows of 2048 bytes: 35.5 us like this, 34 by a warp each; 16384 of 4096: 49 and 64; 4000 of 16 KB: 54 and 88; 300 of 16 KB: 14.5
+        // and 18; 500 of 4096: the same)
+        if (bytes >= 4096 && p.n >= kSms && 2 * stage <= kStreamSmem) {
             int u = 1;
             while (u < 4 && (vecs + u - 1) / u > 256) u *= 2;
             const int threads = ((vecs + u - 1) / u + 31) / 32 * 32;
             if (threads <= 256) {
-                if (u == 1) return launch_norm_grad_stream<T, 1, 256>(s, p, threads, parts);
-                if (u == 2) return launch_norm_grad_stream<T, 2, 256>(s, p, threads, parts);
-                return launch_norm_grad_stream<T, 4, 256>(s, p, threads, parts);
+                // two rows of at most 8 KB each: four stages always fit
+                if (u == 1) return launch_norm_grad_stream<T, 1, 2, 256>(s, p, threads, parts);
+                if (u == 2) return launch_norm_grad_stream<T, 2, 2, 256>(s, p, threads, parts);
+                return launch_norm_grad_stream<T, 4, 1, 256>(s, p, threads, parts);
             }
-            if (threads <= 512) return launch_norm_grad_stream<T, 4, 512>(s, p, threads, parts);
+            if (threads <= 512) return launch_norm_grad_stream<T, 4, 1, 512>(s, p, threads, parts);
         }
     }
     const RowShape r = row_shape(p.dim / VE, VE, p.n);

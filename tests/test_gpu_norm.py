@@ -288,3 +288,43 @@ def test_rows_that_start_anywhere(n, dim, dtype, pad, shift):
     dw2 = torch.zeros_like(dw)
     L.rms_norm_grad(0, dy, x, w, dy, dw2, ws, 1e-5, r)
     assert torch.equal(dy, dx) and torch.equal(dw, dw2)
+
+
+@pytest.mark.parametrize("n,dim,dtype", [(593, 2048, "bf16"), (1185, 2048, "f16"), (1777, 2056, "bf16"), (4001, 1032, "f32"), (741, 4096, "bf16"), (887, 2044, "f32"),
+                                         (1333, 12000, "bf16"), (2000, 8200, "f16"), (607, 16384, "f16"), (893, 5000, "f32"), (592, 8192, "f32")])
+@pytest.mark.parametrize("arrays", [2, 3])
+def test_gradient_of_rows_that_meet_in_pairs(n, dim, dtype, arrays):
+    """Two rows a reduction where the second one may be missing, and wide rows that are read again; the bound is test_gradient's: the root's
+    inverse has one rounding of a product and one of the result, no more than the root and the quotient that it takes the place of."""
+    import torch
+    t = _types()[dtype]
+    x, w, r = _inputs(n, dim, t, torch.float32, arrays == 3, 0, 0, 7)
+    dy = torch.randn(n, dim, device="cuda").to(t)
+    dx, dw = torch.empty_like(dy), torch.zeros(dim, device="cuda")
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda").fill_(0xFF)
+    for turn in range(2):
+        L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 1e-5, r)
+        h, g = x.double(), dy.double() * w.double()
+        s = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+        first, second = s * g, h * s ** 3 * (g * h).mean(1, keepdim=True)
+        extra = r.double() if arrays == 3 else torch.zeros_like(h)
+        mag = first.abs() + h.abs() * s ** 3 * (g * h).abs().mean(1, keepdim=True) + extra.abs()
+        _close(dx, first - second + extra, mag * (130 * U32))
+        terms = dy.double() * h * s
+        _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
+        x.mul_(-0.5)
+    assert L.operator_error(0) == 0
+
+
+@pytest.mark.parametrize("n,dim", [(7, 100), (600, 2048), (600, 12000)])
+def test_gradient_of_rows_without_a_norm(n, dim):
+    """A row of zeros with eps: its gradient is dy w / sqrt(eps).  Squares that sum to infinity: the norm's inverse is 0, and so is the gradient by it."""
+    import torch
+    x = torch.zeros(n, dim, device="cuda")
+    x[1::2] = 3e19
+    w, dy = torch.ones(dim, device="cuda"), torch.full((n, dim), 0.5, device="cuda")
+    dx, dw = torch.empty_like(x), torch.zeros(dim, device="cuda")
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda")
+    L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 2.0 ** -10)
+    assert bool(((dx[0::2] - 16.0).abs() <= 16.0 * 4 * U32).all())
+    assert bool((dx[1::2] == 0).all()) and bool((dw == 0).all())
