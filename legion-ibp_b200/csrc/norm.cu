@@ -3,6 +3,8 @@
 //   h = x + r,   s = 1 / sqrt(mean(h^2) + eps),   y = h * w * s
 //   compressed: a = max |y|, scale = a / top, code = y * (top / a) rounded (the quantiser of the caches; top = 127 or 448)
 //   gradient, g = dy * w:   dx = s * g - h * s^3 * mean(g * h) (+ dres),   dw = sum over rows of dy * h * s
+//   worked out as dx = s * g - (h * s) * (s * (s * mean(g * h))): s^3 is no normal fp32 number for rows below 1.4e-13 and above 4e12,
+//   while h * s and s * mean(g * h) are of the order of 1 and of g whatever the size of the row
 //
 // A row is read once: a group of threads (8 or 32 lanes of a warp, or a CTA) holds it in registers from the loads through
 // the sums to the stores.  s is positive and rounding is monotone, so max |y| is s * max |h * w| to the bit, and the norm
@@ -345,8 +347,10 @@ struct NormGradParams {
     float eps;
 };
 
+// One CTA an SM is asked for where a thread has 32 columns: without that the compiler gives such a thread of fp32 32 registers and 3 KB of
+// spills (2000 rows of 12000 with a residual: 536 us, 113 with 128 registers).
 template <typename T, int VE, int U, int GROUP, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
+__global__ void __launch_bounds__(MAXT, MAXT == 512 && U * VE == 32 ? 1 : 0) norm_grad_kernel(NormGradParams p)
 {
     __shared__ float smem[128];
     __shared__ float cross[GROUP == 0 ? 1 : 128 * U * VE];
@@ -411,16 +415,16 @@ __global__ void __launch_bounds__(MAXT) norm_grad_kernel(NormGradParams p)
         float square = square2.sum(), dot = dot2.sum();
         reduce.two(square, dot, false);
         const float s = inverse_root(fmaf(square, per_dim, p.eps));
-        const float k = s * s * s * (dot * per_dim);
+        const float k = s * (s * (dot * per_dim));
         const Two s2 = Two::of(s, s), k2 = Two::of(-k, -k);
         float dx[2 * P];
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const Two a = pair(h, j), g = pair(dy, j);
-            const Two d = fma(a, k2, fma(g * w[j], s2, pair(r, j)));
+            const Two normed = pair(h, j) * s2, g = pair(dy, j);
+            const Two d = fma(normed, k2, fma(g * w[j], s2, pair(r, j)));
             dx[2 * j] = d.low();
             dx[2 * j + 1] = d.high();
-            if (in) dw[j] = fma(g, a * s2, dw[j]);
+            if (in) dw[j] = fma(g, normed, dw[j]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_grad_stream_kernel(NormGradParam
 #pragma unroll
         for (int q = 0; q < R; ++q) {
             const float s = inverse_root(fmaf(sums[q], per_dim, p.eps));
-            const float k = s * s * s * (sums[R + q] * per_dim);
+            const float k = s * (s * (sums[R + q] * per_dim));
             const Two s2 = Two::of(s, s), k2 = Two::of(-k, -k);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -607,11 +611,11 @@ __global__ void __launch_bounds__(MAXT, 1) norm_grad_stream_kernel(NormGradParam
                 float dx[VE];
 #pragma unroll
                 for (int i = 0; i < VE / 2; ++i) {
-                    const Two a = Two::of(h[q][u].get(2 * i), h[q][u].get(2 * i + 1)), g = Two::of(dy[q][u].get(2 * i), dy[q][u].get(2 * i + 1));
-                    const Two d = fma(a, k2, fma(g * w[u][i], s2, Two::of(r[q][u].get(2 * i), r[q][u].get(2 * i + 1))));
+                    const Two normed = Two::of(h[q][u].get(2 * i), h[q][u].get(2 * i + 1)) * s2, g = Two::of(dy[q][u].get(2 * i), dy[q][u].get(2 * i + 1));
+                    const Two d = fma(normed, k2, fma(g * w[u][i], s2, Two::of(r[q][u].get(2 * i), r[q][u].get(2 * i + 1))));
                     dx[2 * i] = d.low();
                     dx[2 * i + 1] = d.high();
-                    dw[u][i] = fma(g, a * s2, dw[u][i]);
+                    dw[u][i] = fma(g, normed, dw[u][i]);
                 }
                 Vec<T, VE> o;
                 o.set(dx);

@@ -328,3 +328,29 @@ def test_gradient_of_rows_without_a_norm(n, dim):
     L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 2.0 ** -10)
     assert bool(((dx[0::2] - 16.0).abs() <= 16.0 * 4 * U32).all())
     assert bool((dx[1::2] == 0).all()) and bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("n,dim,dtype", [(50, 24, "f32"), (9, 64, "bf16"), (700, 300, "f32"), (20, 4096, "f32"), (30, 1000, "bf16"), (600, 2048, "bf16"), (700, 2052, "f32"),
+                                         (300, 4096, "f32"), (400, 12000, "bf16"), (200, 8192, "f32"), (400, 4097, "f32"), (500, 1027, "bf16")])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-6), (1e17, 1e-6), (1e-14, 0.0), (1e-17, 0.0)])
+def test_gradient_of_large_and_small_rows(n, dim, dtype, size, eps):
+    """Rows whose squares' sum is an fp32 number, while the third power of the norm's inverse is not.  dx = s (dy w - (x s) (s mean(dy w x))), up
+    to the order of the factors: s is off by 25 u, so s twice and x s by 76 u, the mean by 46 u, the products by 5 u: 127 u, within
+    test_gradient's 130 u of the terms' magnitudes."""
+    import torch
+    t = _types()[dtype]
+    torch.manual_seed(dim)
+    x = (torch.randn(n, dim, device="cuda", dtype=torch.float64) * size).to(t)
+    w = 1 + 0.2 * torch.randn(dim, device="cuda")
+    dy = (torch.randn(n, dim, device="cuda") + 2 * x.double().sign()).to(t)   # rows that the second term does not leave alone
+    dx, dw = torch.empty_like(x), torch.zeros(dim, device="cuda")
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda")
+    L.rms_norm_grad(0, dy, x, w, dx, dw, ws, eps)
+    h, g = x.double(), dy.double() * w.double()
+    assert float((h * h).sum(1).max()) < 3.4e38
+    s = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + eps)
+    first, second = s * g, (h * s) * (s * (g * h * s).mean(1, keepdim=True))
+    mag = first.abs() + (h * s).abs() * s * (g * h * s).abs().mean(1, keepdim=True)
+    _close(dx, first - second, mag * (130 * U32))
+    terms = dy.double() * h * s
+    _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
