@@ -416,7 +416,8 @@ int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_t grad_stri
 /* out[i][j] = scale of row i * scale of weight row j * sum over k of their codes' products: m compressed rows (of legion_rms_norm,
  * legion_quantize_table or a cache's partition) times n compressed weight rows (one per output column, for instance
  * legion_quantize_table of an fp32 weight [n][feature_len]), feature_len codes each, both of `codec`.  Strides in bytes, multiples of 16; rows start on
- * multiples of 16 bytes.  int8 products are summed exactly, e4m3 products in fp32; the sum is scaled in fp32 and rounded once.
+ * multiples of 16 bytes.  int8 products are summed exactly, e4m3 products in fp32; the sum is scaled in fp32, by one
+ * scale after the other (their product is not formed), and rounded once.  Results of int8 rows do not depend on the call's other rows.
  * Bytes of a row behind its scale are not read. */
 int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t m, int64_t row_stride, const void *weight_rows,
                        int64_t n, int64_t weight_stride, int32_t feature_len, void *out, int32_t out_dtype, int64_t out_stride,

@@ -207,3 +207,42 @@ def test_nothing_to_do_and_refusals():
     with pytest.raises(L.LegionError, match="limit"):
         L.matmul_rows(0, 1, long, long, 131072, torch.zeros(1, 1, device="cuda"))
     assert bool((out == 3.0).all())
+
+
+@pytest.mark.parametrize("codec", CODECS)
+def test_scales_far_from_one(codec):
+    """Scales whose product leaves fp32's range while the result does not, at every number of rows that is served in a way of its own: each
+    result is the sum scaled, and int8 rows (whose sums are exact) give the same bits whatever other rows are in the call.  The sum meets the
+    row's scale first, above 2^92 the weight's: a whole number times a subnormal one is exact or normal, so the three roundings of _check are all
+    (e4m3 sums are multiples of 2^-18: scales from 1e-30 on keep them normal)."""
+    import torch
+    n, k, most = 1280, 64, 3712
+    a, b = _coded(most, k, codec, 0, 11), _coded(n, k, codec, 0, 12)
+    a[0][::7, :k] = 0
+    a[1][::7] = 0
+    low = -44.0 if codec == L.CODEC_INT8 else -30.0
+    scales = []
+    for rows in (a, b):
+        s = (10.0 ** (low + (30.0 - low) * torch.rand(rows[0].shape[0], device="cuda", dtype=torch.float64))).float()
+        s[0], s[1], s[2] = 1e25, 1e-22, 1e-23
+        rows[0].view(torch.float32)[:, k // 4] = s
+        scales.append(s.double())
+    sums, outer = a[1] @ b[1].t(), scales[0][:, None] * scales[1][None]
+    want = sums * outer
+    slack = want.abs() * (3 * U32)
+    if codec == L.CODEC_E4M3:
+        slack = slack + (a[1].abs() @ b[1].abs().t()) * outer * (k * 2 * U32)
+    over = want.abs() > 3.4e38
+    near = over | (want.abs() + slack > 3.4e38)
+    whole = None
+    for m in (most, 2500, 1500, 300, 100, 50, 20, 9, 1):
+        out = torch.empty(m, n, device="cuda")
+        L.matmul_rows(0, codec, a[0][:m], b[0], k, out)
+        assert not bool(torch.isnan(out).any())
+        assert torch.equal(torch.isinf(out) | near[:m], near[:m])
+        _close(torch.where(near[:m], 0.0, out), torch.where(near[:m], 0.0, want[:m]), torch.where(near[:m], 0.0, slack[:m]))
+        assert bool((out[::7] == 0).all())
+        if codec == L.CODEC_INT8:
+            whole = out if whole is None else whole
+            assert torch.equal(out, whole[:m])
+    assert int(over.sum()) > 0
