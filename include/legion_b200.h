@@ -425,6 +425,10 @@ int legion_matmul_rows(int32_t dev_id, int32_t codec, const void *rows, int64_t 
 /* First error that a kernel of these operators raised on dev_id since the last reset (0: none; LEGION_E_TIMEOUT: a copy or a product
  * inside legion_matmul_rows or legion_rms_norm_grad did not complete within its wait limit, the call's output is not valid).  Waits for `stream`. */
 int legion_operator_error(int32_t dev_id, void *stream, int32_t *error, int32_t reset);
+/* How long a wait inside a kernel of legion_matmul_rows or legion_rms_norm_grad may last before it is given up (2 seconds unless set; at most 60),
+ * for the calls that this process makes from now on; a captured graph keeps the limit of its capture.  0: as if every wait had been given up, for
+ * tests of what a caller does then. */
+int legion_operator_wait_limit(int64_t microseconds);
 
 /* The operators above with their arguments in one block, for bindings that pay per argument (a ctypes call costs 0.1 us for each).  A block
  * begins with the operator's number and its own size in bytes; its fields are the call's arguments, 8-byte ones first, without padding. */

@@ -381,6 +381,7 @@ def _declare_operators(l):
     l.legion_rms_norm_grad_workspace.argtypes = [Q, I, P]
     l.legion_matmul_rows.argtypes = [I, I, P, Q, Q, P, Q, Q, I, P, I, Q, P]
     l.legion_operator_error.argtypes = [I, P, P, I]
+    l.legion_operator_wait_limit.argtypes = [Q]
     l.legion_operator_call.argtypes = [C.c_char_p]
 
 
@@ -593,6 +594,12 @@ def operator_error(dev_id, stream=None, reset=True):
     e = C.c_int32()
     _check(lib().legion_operator_error(dev_id, None if stream is None else _handle(stream), C.byref(e), 1 if reset else 0))
     return e.value
+
+
+def operator_wait_limit(microseconds):
+    """How long a wait inside a kernel of these operators may last, for calls made from now on (2,000,000 unless set).  One that
+    is given up leaves LEGION_E_TIMEOUT (-7) in operator_error; 0 gives up every wait, for tests of what follows."""
+    _check(lib().legion_operator_wait_limit(microseconds))
 
 
 class IPCEnv:

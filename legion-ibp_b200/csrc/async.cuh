@@ -18,8 +18,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// Waits until the barrier's phase of that parity is over: at most `tries` times 20 microseconds (kWaitTries: two seconds), then false.
-constexpr uint32_t kWaitTries = 100000;
+// Waits until the barrier's phase of that parity is over: at most `tries` times kTryUs microseconds (once, where tries is 0), then false.
+constexpr int kTryUs = 20;
 __device__ __forceinline__ bool wait_barrier(uint32_t bar, uint32_t parity, uint32_t tries)
 {
     uint32_t ok;
@@ -42,6 +42,9 @@ inline int allow_smem(const void *kernel, int bytes, bool *done)
     }
     return LEGION_OK;
 }
+
+// Tries of a wait inside a launch made now (legion_operator_wait_limit): two seconds' worth, unless the caller has set another limit.
+uint32_t operator_wait_tries();
 
 // Kernels of two files raise errors, each in a word of its own file's (legion_operator_error reads both).
 cudaError_t norm_error_word(void **word);

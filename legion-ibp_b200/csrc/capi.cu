@@ -1,6 +1,7 @@
 // C ABI: storage handles, the memory pool, the five operators and the whole-batch calls.
-#include "common.cuh"
+#include "async.cuh"
 
+#include <atomic>
 #include <stdarg.h>
 #include <string.h>
 
@@ -543,6 +544,18 @@ extern "C" int legion_enable_peer_access(int32_t dev_id, int32_t peer_id)
         return LEGION_OK;
     }
     LG_CUDA(e);
+    return LEGION_OK;
+}
+
+// ---- operators on learned and compressed rows: how long their kernels wait ------------------------------------------------
+
+static std::atomic<uint32_t> g_wait_tries{ 2000000 / kTryUs };
+uint32_t legion::operator_wait_tries() { return g_wait_tries.load(std::memory_order_relaxed); }
+
+extern "C" int legion_operator_wait_limit(int64_t microseconds)
+{
+    LG_ARG(microseconds >= 0 && microseconds <= 60000000, "the limit of a wait is 0 to 60 seconds");
+    g_wait_tries.store((uint32_t)((microseconds + kTryUs - 1) / kTryUs), std::memory_order_relaxed);
     return LEGION_OK;
 }
 

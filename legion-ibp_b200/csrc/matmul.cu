@@ -130,6 +130,7 @@ struct MatmulParams {
     int32_t word;     // the widest word of 16, 8, 4 or 2 bytes that the output's rows start on multiples of
     int32_t stages, stage_bytes, q_at;   // of shared memory; where a stage's rows of Q begin
     int32_t step_p;   // rows of P per CTA and tile: kTileP, or fewer (a multiple of 8) where that gives every SM a tile
+    uint32_t tries;   // of a wait
 };
 
 constexpr int kTileP = 128;
@@ -385,7 +386,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
 
     if (warp == 4 || warp == 6) {
         if (PAIR == 2) full_of_first = in_first_cta(full);
-        uint32_t tries = kWaitTries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
+        uint32_t tries = m.tries;   // after a wait that was given up the others are not waited for: the loops end, the call has failed
         while (tile < tiles) {
             if (!wait_barrier(empty + 8 * stage, (round & 1) ^ 1, tries)) tries = 0;
             if (__any_sync(kFull, tries == 0)) break;
@@ -411,7 +412,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             const uint64_t first = operand_desc(shared_addr(smem));
             const uint32_t stage16 = (uint32_t)kStage >> 4, sub16 = sub_bytes >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
             int s = 0, turn = 0;
-            uint32_t around = 0, tries = kWaitTries;
+            uint32_t around = 0, tries = m.tries;
             for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
                 if (!wait_barrier(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
@@ -456,7 +457,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 qs[i] = q < m.q_n ? *reinterpret_cast<const float *>(m.q_rows + (int64_t)q * m.q_stride + m.k) : 0.0f;
             }
             const float ps = mine ? *reinterpret_cast<const float *>(m.p_rows + (int64_t)p * m.p_stride + m.k) : 0.0f;
-            if (!wait_barrier(acc_full + 8 * a, (turn >> 1) & 1, kWaitTries)) *gave_up = 1;
+            if (!wait_barrier(acc_full + 8 * a, (turn >> 1) & 1, m.tries)) *gave_up = 1;
             if (any_of_128(*gave_up != 0)) break;   // all four warps go on, or none; also: the scales are there
             fence_after();
             const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + a * BQ;
@@ -669,8 +670,8 @@ template <int CODEC>
 static int launch_matmul(cudaStream_t s, const uint8_t *rows, int64_t m, int64_t row_stride, const uint8_t *weights, int64_t n,
                          int64_t weight_stride, int32_t k, void *out, int32_t out_dtype, int64_t out_stride)
 {
-    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0, 0, 0, 0, weights_per_cta(n) };
-    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0, 0, 0, 0, kTileP };
+    const MatmulParams by_weight{ weights, rows, weight_stride, row_stride, (int32_t)n, (int32_t)m, k, out, out_stride, out_dtype, 0, 0, 0, 0, weights_per_cta(n), operator_wait_tries() };
+    const MatmulParams by_row{ rows, weights, row_stride, weight_stride, (int32_t)m, (int32_t)n, k, out, out_stride, out_dtype, 0, 0, 0, 0, kTileP, operator_wait_tries() };
     if (m == 1) {
         matvec_kernel<CODEC, 2><<<(unsigned)((n + 15) / 16), 256, 0, s>>>(by_weight);
         LG_LAUNCH_CHECK();

@@ -345,6 +345,7 @@ struct NormGradParams {
     int64_t n, grad_stride, x_stride, grad_residual_stride, grad_x_stride;
     int32_t dim, weight_dtype;
     float eps;
+    uint32_t tries;   // of a wait
 };
 
 // One CTA an SM is asked for where a thread has 32 columns: without that the compiler gives such a thread of fp32 32 registers and 3 KB of
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_grad_stream_kernel(NormGradParam
     const float per_dim = 1.0f / (float)p.dim;
     __syncthreads();
     int stage = 0;
-    uint32_t phase = 0, tries = kWaitTries;
+    uint32_t phase = 0, tries = p.tries;
     for (int64_t row = blockIdx.x; row < p.n; row += R * step) {
         Vec<T, VE> h[R][U], dy[R][U], r[R][U];
         const uint8_t *src[R];
@@ -638,11 +639,11 @@ __global__ void __launch_bounds__(MAXT, 1) norm_grad_stream_kernel(NormGradParam
         o.set(x);
         o.store(part + col);
     }
-    if (tries == 0) {
+    // one thread's wait may have been given up where another's was not: all of them decide together
+    if (__syncthreads_or(tries == 0) && t == 0) {
         raise_operator_error();
-        if (t == 0)   // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
-            for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
-        __syncthreads();
+        // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
+        for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
     }
 }
 
@@ -974,7 +975,7 @@ extern "C" int legion_rms_norm_grad(int32_t dev_id, const void *grad_out, int64_
         return LEGION_OK;
     }
     NormGradParams p{ grad_out, x, grad_residual, weight, grad_x, (float *)workspace, n_rows, grad_stride, x_stride, grad_residual_stride,
-                      grad_x_stride, dim, weight_dtype, eps };
+                      grad_x_stride, dim, weight_dtype, eps, operator_wait_tries() };
     int ve = common_vector(dtype == LEGION_F32 ? 4 : 8, { dim, x_stride, aligned_elements(x, dtype), grad_stride, aligned_elements(grad_out, dtype),
                                                           grad_x_stride, aligned_elements(grad_x, dtype) });
     if (grad_residual != nullptr) ve = common_vector(ve, { grad_residual_stride, aligned_elements(grad_residual, dtype) });

@@ -354,3 +354,37 @@ def test_gradient_of_large_and_small_rows(n, dim, dtype, size, eps):
     _close(dx, first - second, mag * (130 * U32))
     terms = dy.double() * h * s
     _close(dw, terms.sum(0), terms.abs().sum(0) * ((n + 32) * U32))
+
+
+@pytest.fixture
+def wait_limit():
+    yield L.operator_wait_limit
+    L.operator_wait_limit(2000000)
+
+
+@pytest.mark.parametrize("n,dim,dtype", [(8000, 2048, "bf16"), (3000, 4096, "f32"), (3000, 12000, "bf16")])
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_wait_that_is_given_up(wait_limit, n, dim, dtype, residual):
+    """Limit 0: the rows behind the first stages are never brought, their waits run out, and the call ends with its error; limits about as long as a
+    copy takes: the waits of some threads of a CTA may run out and those of others not, and the call ends with an error or is right."""
+    import torch
+    t = _types()[dtype]
+    x, w, r = _inputs(n, dim, t, torch.float32, residual, 0, 0, 3)
+    dy = torch.randn(n, dim, device="cuda").to(t)
+    ws = torch.empty(L.rms_norm_grad_workspace(n, dim), dtype=torch.uint8, device="cuda")
+    want, want_w = torch.empty_like(dy), torch.zeros(dim, device="cuda")
+    L.rms_norm_grad(0, dy, x, w, want, want_w, ws, 1e-5, r)
+    assert L.operator_error(0) == 0
+    for limit in (0, 1, 20, 40, 200):
+        wait_limit(limit)
+        dx, dw = torch.empty_like(dy), torch.zeros(dim, device="cuda")
+        L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 1e-5, r)
+        error = L.operator_error(0, reset=False)
+        assert error == (-7 if limit == 0 else error) and error in (0, -7)
+        assert L.operator_error(0) == error and L.operator_error(0) == 0   # kept until it is reset
+        if error == 0:
+            assert torch.equal(dx, want) and torch.equal(dw, want_w)
+    wait_limit(2000000)
+    dx, dw = torch.empty_like(dy), torch.zeros(dim, device="cuda")
+    L.rms_norm_grad(0, dy, x, w, dx, dw, ws, 1e-5, r)
+    assert L.operator_error(0) == 0 and torch.equal(dx, want) and torch.equal(dw, want_w)

@@ -105,3 +105,14 @@ def test_workspace_sizes():
             bad()
     b = C.c_int64()
     assert L.lib().legion_embedding_grad_workspace(1, 8, 10, None) == -1 and L.lib().legion_rms_norm_grad_workspace(1, 8, C.byref(b)) == 0
+
+
+def test_limits_of_waits():
+    try:
+        for good in (0, 1, 60000000):
+            L.operator_wait_limit(good)
+        for bad in (-1, 60000001):
+            with pytest.raises(L.LegionError):
+                L.operator_wait_limit(bad)
+    finally:
+        L.operator_wait_limit(2000000)
