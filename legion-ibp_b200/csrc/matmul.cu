@@ -400,10 +400,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                 ++round;
             }
         }
-        if (tries == 0) {  // the copies that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
-            *gave_up = 1;
-            for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
-        }
+        if (tries == 0) *gave_up = 1;
     } else if (warp == 5) {
         if (me == 0) {
             // The whole warp walks through the stages and one lane of it issues: what the products are issued with stays uniform
@@ -412,14 +409,17 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
             const uint64_t first = operand_desc(shared_addr(smem));
             const uint32_t stage16 = (uint32_t)kStage >> 4, sub16 = sub_bytes >> 4, q16 = (uint32_t)q_at >> 4;   // descriptors count in 16 bytes
             int s = 0, turn = 0;
-            uint32_t around = 0, tries = m.tries;
+            uint32_t around = 0;
+            bool over = false;   // a wait was given up: nothing more is issued
             for (int64_t t = blockIdx.x / PAIR; t < tiles; t += gridDim.x / PAIR, ++turn) {
                 const int a = turn & 1;
-                if (!wait_barrier(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, tries)) tries = 0;
+                over = __any_sync(kFull, !wait_barrier(acc_empty + 8 * a, ((turn >> 1) & 1) ^ 1, m.tries));
+                if (over) break;
                 fence_after();
                 const uint32_t acc = tmem + a * BQ;
                 for (int kb = 0; kb < blocks_k; kb += kSub) {
-                    if (!wait_barrier(full + 8 * s, around & 1, tries)) tries = 0;
+                    over = __any_sync(kFull, !wait_barrier(full + 8 * s, around & 1, m.tries));
+                    if (over) break;
                     const uint64_t dp = first + (uint32_t)s * stage16;
                     const int left = m.k - kb * kTileK;   // 32 codes a product; the last block has as many as the rows reach into
                     if (one_lane()) {
@@ -437,9 +437,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
                         ++around;
                     }
                 }
-                if (__any_sync(kFull, tries == 0)) break;
+                if (over) break;
             }
-            if (tries == 0) *gave_up = 1;
+            if (over) *gave_up = 1;
         }
     } else {
         const uint32_t acc_empty_of_first = PAIR == 2 ? in_first_cta(acc_empty) : acc_empty;
@@ -484,6 +484,10 @@ matmul_kernel(const __grid_constant__ CUtensorMap p_map, const __grid_constant__
     __syncwarp();
     fence_before();
     __syncthreads();
+    if (*gave_up) {   // the copies and products that are under way land before the CTA's memory goes: they take microseconds, this waits a millisecond
+        for (const long long t0 = clock64(); clock64() - t0 < 2000000;) { }
+        __syncwarp();
+    }
     if (PAIR == 2) pair_sync();   // nothing of the other CTA still signals here, and the products that wrote its TMEM are done
     fence_after();
     if (threadIdx.x == 0 && *gave_up) atomicCAS(&g_operator_error, 0, LEGION_E_TIMEOUT);

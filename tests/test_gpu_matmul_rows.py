@@ -246,3 +246,30 @@ def test_scales_far_from_one(codec):
             whole = out if whole is None else whole
             assert torch.equal(out, whole[:m])
     assert int(over.sum()) > 0
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 64), (20, 1280, 4100), (100, 40, 260), (300, 1280, 4100), (1500, 1280, 64), (2500, 1280, 2052), (3712, 1280, 1028), (2500, 9001, 132)])
+@pytest.mark.parametrize("codec", CODECS)
+def test_a_wait_that_is_given_up(codec, m, n, k):
+    """Limit 0: nothing is brought, the waits for it run out, and the call ends with its error; limits about as long as a tile takes: some waits may
+    run out and others not, and the call ends with an error or is right.  (One row is worked out without waits.)"""
+    import torch
+    a, b = _coded(m, k, codec, 0, 1), _coded(n, k, codec, 0, 2)
+    want = torch.empty(m, n, device="cuda")
+    L.matmul_rows(0, codec, a[0], b[0], k, want)
+    assert L.operator_error(0) == 0
+    try:
+        for limit in (0, 1, 20, 40, 100, 300):
+            L.operator_wait_limit(limit)
+            out = torch.empty(m, n, device="cuda")
+            L.matmul_rows(0, codec, a[0], b[0], k, out)
+            error = L.operator_error(0, reset=False)
+            assert error in ((0,) if m == 1 else (-7,) if limit == 0 else (0, -7))
+            assert L.operator_error(0) == error and L.operator_error(0) == 0   # kept until it is reset
+            if error == 0:
+                assert torch.equal(out, want)
+    finally:
+        L.operator_wait_limit(2000000)
+    out = torch.empty(m, n, device="cuda")
+    L.matmul_rows(0, codec, a[0], b[0], k, out)
+    assert L.operator_error(0) == 0 and torch.equal(out, want)
