@@ -331,3 +331,17 @@ def test_refusals():
                 lambda: L.embedding_grad_rows(0, ids, out, 5, ids.long(), out, ids[:1], torch.zeros(1 << 20, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(L.LegionError):
             bad()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), -2.0, float("nan")])
+@pytest.mark.parametrize("n,dim,dtype", [(5, 64, "f32"), (3000, 128, "bf16"), (50, 333, "f16"), (9, 7, "f32")])
+def test_lookup_outside_the_table_is_zero_whatever_the_scale(n, dim, dtype, scale):
+    import torch
+    t = _types()[dtype]
+    table = torch.ones(10, dim, dtype=t, device="cuda")
+    ids = torch.arange(n, device="cuda") % 12 - 1   # -1 and 10 among them
+    out = torch.full((n, dim), 3.0, dtype=t, device="cuda")
+    L.embedding_lookup(0, table, ids, out, scale)
+    none = (ids < 0) | (ids > 9)
+    assert bool((out[none].view(torch.int32 if dtype == "f32" else torch.int16) == 0).all())
+    assert torch.equal(out[~none].nan_to_num(7.0), torch.full_like(out[~none], scale).nan_to_num(7.0))
