@@ -345,3 +345,40 @@ def test_lookup_outside_the_table_is_zero_whatever_the_scale(n, dim, dtype, scal
     none = (ids < 0) | (ids > 9)
     assert bool((out[none].view(torch.int32 if dtype == "f32" else torch.int16) == 0).all())
     assert torch.equal(out[~none].nan_to_num(7.0), torch.full_like(out[~none], scale).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("n", [0, 40, 5000, 30000])
+def test_gradient_of_a_table_with_far_rows(n):
+    """Rows of the table that lie more than 2^31 bytes apart."""
+    import torch
+    nodes, dim, stride = 2, 64, (1 << 29) + 64
+    whole = torch.full((stride + dim,), 7.0, device="cuda")
+    out = torch.as_strided(whole, (nodes, dim), (stride, 1))
+    ids, grad = torch.ones(n, dtype=torch.int32, device="cuda"), torch.ones(n, dim, device="cuda")
+    ws = torch.empty(L.embedding_grad_workspace(n, dim, nodes), dtype=torch.uint8, device="cuda")
+    L.embedding_grad(0, ids, grad, out, ws)
+    assert bool((out[0] == 0).all()) and bool((out[1] == n).all())   # whole numbers: exact
+    assert bool((whole[dim:stride] == 7.0).all())
+
+
+@pytest.mark.parametrize("n,nodes,dim", [((1 << 20) + 5, 70000, 3), ((1 << 22) + 3, 1 << 20, 2), (30001, (1 << 24) + 9, 3)])
+def test_gradient_of_the_longest_lists_and_largest_tables(n, nodes, dim):
+    """Stretches of 64 and of 128 entries, four passes over long lists."""
+    import torch
+    rng = np.random.default_rng(n)
+    ids = _ids(rng, n, nodes, False, 2.0)
+    ids[5], ids[77] = -1, nodes
+    grad = torch.randn(n, dim, device="cuda")
+    want, mag, count = _exact_grad(ids, grad, nodes, 1.0)
+    ws = torch.empty(L.embedding_grad_workspace(n, dim, nodes), dtype=torch.uint8, device="cuda").fill_(0xA5)
+    out = torch.full((nodes, dim), 3.0, device="cuda")
+    L.embedding_grad(0, ids, grad, out, ws)
+    _close(out, want, mag * ((count[:, None] + 2).double() * U32))
+    unique, rows = torch.full((n,), -9, dtype=torch.int32, device="cuda"), torch.full((n, dim), -9.0, device="cuda")
+    found = torch.zeros(1, dtype=torch.int32, device="cuda")
+    L.embedding_grad_rows(0, ids, grad, nodes, unique, rows, found, ws)
+    occur = torch.nonzero(count).flatten()
+    k = occur.numel()
+    assert int(found) == k and torch.equal(unique[:k].long(), occur)
+    assert torch.equal(rows[:k], out[occur])   # the same sums in the same order
+    assert bool((unique[k:] == -9).all()) and bool((rows[k:] == -9.0).all())
