@@ -246,18 +246,22 @@ __device__ __forceinline__ void store_tile(uint32_t acc, float ps, const float *
                 o.store(reinterpret_cast<T *>(row + (((half + i) / kPer16) ^ (lane & 7)) * 16));
             }
         }
-        if (m.word == 16) {
+        const int cols = min(kCols, m.q_n - q0 - c);
+        if (m.word == 16 && cols % kPer16 == 0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) tma_store_2d(map, shared_addr(row), q0 + c, p0);
-        } else {   // rows that TMA cannot address: the lanes write along them, in words that the rows start on
+        } else {
+            // Rows that TMA cannot address, or that end inside 16 bytes (TMA leaves out what lies behind a row's end by whole 16 bytes only and zeroes
+            // the rest): the lanes write along them, in words that the rows start on.
             __syncwarp();
-            const int rows = min(32, m.p_n - p0), cols = min(kCols, m.q_n - q0 - c);
+            const int rows = min(32, m.p_n - p0);
             T *dst = static_cast<T *>(m.out) + (int64_t)p0 * m.out_stride + q0 + c;
             const uint8_t *src = row - lane * 128;
-            if (m.word == 8) write_rows<uint2, T, kCols, true>(dst, m.out_stride, src, rows, cols);
+            if (m.word >= 8) write_rows<uint2, T, kCols, true>(dst, m.out_stride, src, rows, cols);
             else if (m.word == 4) write_rows<uint32_t, T, kCols, true>(dst, m.out_stride, src, rows, cols);
             else write_rows<uint16_t, T, kCols, true>(dst, m.out_stride, src, rows, cols);
+            if (m.word == 16 && lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // of no copies: the wait above counts a group a buffer
             __syncwarp();
         }
     }
@@ -602,7 +606,7 @@ static int make_map(CUtensorMap *map, const void *rows, int64_t n, int64_t strid
     return LEGION_OK;
 }
 
-// boxes of 32 rows, 128 bytes of each; what lies outside of the output is not written
+// boxes of 32 rows, 128 bytes of each; what lies outside of the output is not written, behind a row's end by whole 16 bytes (store_tile sees to the rest)
 static int make_out_map(CUtensorMap *map, const MatmulParams &m)
 {
     EncodeTiled encode = encode_tiled();

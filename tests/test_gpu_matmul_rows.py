@@ -273,3 +273,31 @@ def test_a_wait_that_is_given_up(codec, m, n, k):
     out = torch.empty(m, n, device="cuda")
     L.matmul_rows(0, codec, a[0], b[0], k, out)
     assert L.operator_error(0) == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("codec", CODECS)
+@pytest.mark.parametrize("out_type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 20, 100, 131, 300, 1500, 2500, 3712])
+@pytest.mark.parametrize("n", [1, 5, 66, 265, 1001, 1279, 1283])
+def test_rows_that_end_inside_16_bytes(codec, out_type, m, n):
+    """Rows of the output that start on 16-byte boundaries, whatever their length: what lies between them stays as it was."""
+    import torch
+    t, k = _types()[out_type], 64
+    per = 16 // t.itemsize
+    for pad in (-n % per, -n % per + per):
+        a, b = _coded(m, k, codec, 0, 21), _coded(n, k, codec, 0, 22)
+        a = (a[0], a[1], a[2] / 4096)
+        a[0].view(torch.float32)[:, k // 4] = a[2].float()
+        whole, out = _strided(m, n, t, pad, 0)
+        L.matmul_rows(0, codec, a[0], b[0], k, out)
+        # fp16: what lies beyond the type's largest number, whose last binade has steps of 2^-10, is infinite or that number
+        want = (a[1] @ b[1].t()) * a[2][:, None] * b[2][None]
+        over = want.abs() > torch.finfo(t).max * (1 - 2 ** -11)
+        assert bool((out[over].abs() >= torch.finfo(t).max * (1 - 2 ** -10)).all())
+        slack = want.abs() * (3 * U32)
+        if codec == L.CODEC_E4M3:
+            slack = slack + (a[1].abs() @ b[1].abs().t()) * a[2][:, None] * b[2][None] * (k * 2 * U32)
+        _close(torch.where(over, 0.0, out), torch.where(over, 0.0, want), torch.where(over, 0.0, slack))
+        rest = whole.clone()
+        torch.as_strided(rest, (m, n), (n + pad, 1), 0).fill_(7.0)
+        assert bool((rest == 7.0).all())
