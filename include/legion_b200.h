@@ -354,7 +354,8 @@ int legion_gather_rows_noalloc(void *stream, int32_t dev_id, const int32_t *ids_
 /* ---- learned rows, norm and products ------------------------------------------------------------------ */
 
 /* Operators that a model needs next to the rows served above: lookup of learned rows with its gradient, RMS norm
- * with its gradient, and products of compressed rows.  They work on device memory of dev_id, in the order of `stream`,
+ * with its gradient, and products of compressed rows.  They work on device memory of dev_id, in the order of `stream` (NULL: the
+ * legacy default stream),
  * allocate nothing, keep nothing between calls, do not synchronise, may be captured into a CUDA graph (make a first call on the device
  * before the capture, as code is loaded with it), and leave the calling thread's current device as it was.  Calls on different streams may run at the same time as long as they do
  * not share a workspace or an output.  Rows are rows of dim elements; strides are in elements (compressed rows: in bytes) and may be
@@ -370,7 +371,8 @@ int legion_gather_rows_noalloc(void *stream, int32_t dev_id, const int32_t *ids_
 #define LEGION_NORM_MAX_DIM (1 << 14)
 #define LEGION_MATMUL_MAX_DIM 131068 /* sums of products of two codes stay inside 32 bits */
 
-/* out[i] = scale * table[ids[i]], computed in fp32 and rounded once; an id outside [0, n_nodes) gives a row of zeros.
+/* out[i] = scale * table[ids[i]], computed in fp32 and rounded once; an id outside [0, n_nodes) gives a row of zeros, whatever the scale.  More
+ * than 2^40 elements in a call are refused (LEGION_E_LIMIT).
  * ids: n_ids values of id_bytes (4 or 8) on the device; any id may come any number of times.  The gather of given rows is
  * FeatureCacheLookup (engine/operator_impl.cuh:39-53); learned rows have no counterpart in the reference. */
 int legion_embedding_lookup(int32_t dev_id, const void *table, int32_t table_dtype, int64_t table_stride, int64_t n_nodes,
@@ -404,7 +406,8 @@ int legion_rms_norm(int32_t dev_id, const void *x, int32_t dtype, int64_t x_stri
                     int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps, int64_t n_rows, int32_t dim,
                     int32_t codec, void *out, int64_t out_stride, void *residual_out, int64_t residual_out_stride, void *stream);
 int legion_rms_norm_grad_workspace(int64_t n_rows, int32_t dim, int64_t *bytes);
-/* The norm's gradient.  x: the rows that were normed (with a residual: residual_out).  grad_x = the gradient of x by way of out, plus
+/* The norm's gradient.  x: the rows that were normed (with a residual: residual_out, which in fp16 and bf16 is the sum rounded, where the norm took the
+ * sum itself: the gradient is that at the rounded rows).  Sums of squares and of grad_out * weight * x are fp32.  grad_x = the gradient of x by way of out, plus
  * grad_residual (the gradient that reached residual_out otherwise; may be NULL); with a residual it is the gradient
  * of both.  grad_weight (dim elements, fp32 or the rows' type) is set, not added to.  grad_x may be grad_out, x or grad_residual (same address and
  * stride).  Workspace as above. */

@@ -366,6 +366,9 @@ def gather_rows_noalloc(stream, dev_id, ids_dev, lut_ptr, capacity, kg, ki, part
 
 
 # ---- learned rows, norm and products ------------------------------------------------------------------
+# stream: a torch stream or its handle.  None is the legacy default stream, not torch's current one: a call between torch operations on another
+# stream names it (stream=torch.cuda.current_stream()).  autograd does not see these calls: a torch.autograd.Function around them makes the
+# forward call in its forward() and the gradient's call, on the stream that is current there, in its backward().
 
 def _declare_operators(l):
     """Argument types of the operators that are called once per layer.  The six that compute are called by legion_operator_call with
@@ -461,7 +464,7 @@ def _handle(stream):
 
 def embedding_lookup(dev_id, table, ids, out, scale=1.0, stream=None):
     """out[i] = scale * table[ids[i]] for a table [nodes, dim] of learned rows; an id outside the table gives a row of zeros.
-    table and out: float32, float16 or bfloat16, each its own; ids: int32 or int64."""
+    table and out: float32, float16 or bfloat16, each its own; ids: int32 or int64.  stream None: the legacy default stream."""
     td, ts = _rows("table", table, dev_id)
     width = _id_width("ids", ids, dev_id)
     n, (nodes, dim) = ids.shape[0], table.shape
@@ -482,7 +485,7 @@ def embedding_grad_workspace(n_ids, dim, n_nodes):
 
 def embedding_grad(dev_id, ids, grad_out, grad_table, workspace, scale=1.0, accumulate=False, stream=None):
     """grad_table[v] = scale * sum of grad_out[i] over ids[i] == v, or added to what grad_table holds.  Ids outside the table
-    are left out."""
+    are left out.  stream None: the legacy default stream."""
     width = _id_width("ids", ids, dev_id)
     td, ts = _rows("grad_table", grad_table, dev_id)
     n, (nodes, dim) = ids.shape[0], grad_table.shape
@@ -497,7 +500,7 @@ def embedding_grad(dev_id, ids, grad_out, grad_table, workspace, scale=1.0, accu
 
 def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, count, workspace, scale=1.0, stream=None):
     """The gradient's rows that occur: unique_ids[:count] rising, grad_rows[:count] their float32 gradients; count is one
-    int32 on the device.  What lies behind count is left as it was."""
+    int32 on the device.  What lies behind count is left as it was.  stream None: the legacy default stream."""
     width = _id_width("ids", ids, dev_id)
     gd, gs = _rows("grad_out", grad_out, dev_id)
     n, dim = grad_out.shape
@@ -520,7 +523,7 @@ def embedding_grad_rows(dev_id, ids, grad_out, n_nodes, unique_ids, grad_rows, c
 
 def rms_norm(dev_id, x, weight, out, eps=1e-6, residual=None, residual_out=None, codec=CODEC_RAW, stream=None):
     """h = x + residual; out = h * weight / sqrt(mean(h^2) + eps); residual_out = h.  codec CODEC_INT8 or CODEC_E4M3: out is uint8
-    and receives the compressed rows that quantize_table would make of the float32 result."""
+    and receives the compressed rows that quantize_table would make of the float32 result.  stream None: the legacy default stream."""
     dt, xs = _rows("x", x, dev_id)
     shape = n, dim = x.shape
     wd = _operand("weight", weight, dev_id, 1, (dim,))[0]
@@ -556,7 +559,7 @@ def rms_norm_grad_workspace(n_rows, dim):
 
 def rms_norm_grad(dev_id, grad_out, x, weight, grad_x, grad_weight, workspace, eps=1e-6, grad_residual=None, stream=None):
     """Gradients of rms_norm at the rows x that were normed (its residual_out, if it had a residual).  grad_residual: what reached
-    residual_out by other ways, added to grad_x."""
+    residual_out by other ways, added to grad_x.  stream None: the legacy default stream."""
     dt, xs = _rows("x", x, dev_id)
     shape = n, dim = x.shape
     gd, gs = _rows("grad_out", grad_out, dev_id, shape)
@@ -578,7 +581,8 @@ def rms_norm_grad(dev_id, grad_out, x, weight, grad_x, grad_weight, workspace, e
 
 def matmul_rows(dev_id, codec, rows, weight_rows, feature_len, out, stream=None):
     """out[i, j] = sum over the codes of row i and weight row j, times both rows' scales.  rows, weight_rows: uint8, compressed rows of
-    feature_len codes (rms_norm, quantize_table, a cache's partition); out: float32, float16 or bfloat16."""
+    feature_len codes (rms_norm, quantize_table, a cache's partition); out: float32, float16 or bfloat16.  stream None: the legacy
+    default stream."""
     rs, ws = _code_rows("rows", rows, dev_id, feature_len), _code_rows("weight_rows", weight_rows, dev_id, feature_len)
     m, n = rows.shape[0], weight_rows.shape[0]
     od, os_ = _rows("out", out, dev_id, (m, n))
